@@ -15,7 +15,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libdramattn.so"
 
-DA_F32, DA_F16, DA_BF16 = 0, 1, 2
+DA_F32, DA_F16, DA_BF16, DA_E4M3 = 0, 1, 2, 3
 DA_I32, DA_I64 = 0, 1
 DA_TIME_F32, DA_TIME_I32 = 0, 1
 
@@ -24,7 +24,7 @@ _ITYPES = {torch.int32: DA_I32, torch.int64: DA_I64}
 _TIME_TYPES = {torch.float32: DA_TIME_F32, torch.int32: DA_TIME_I32}
 
 # name -> (restype, argtypes); one line per symbol of the header (those that _host calls natively, da_decode_attention,
-# da_linear_qkv_rope and da_linear_block_tail, are for other callers here)
+# da_linear_qkv_rope, da_linear_block_tail, da_rotate, da_paged_append and da_paged_attention, are for other callers here)
 SIGNATURES = {
     "da_version": (c_int, []),
     "da_last_error_string": (c_char_p, []),
@@ -142,6 +142,10 @@ SIGNATURES = {
         c_int,
         [c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p,
          c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "da_rotate": (c_int, [c_char_p, c_size_t, c_void_p]),
+    "da_paged_append": (c_int, [c_char_p, c_size_t, c_void_p]),
+    "da_paged_attention_workspace_bytes": (c_size_t, [c_char_p, c_size_t]),
+    "da_paged_attention": (c_int, [c_char_p, c_size_t, c_void_p]),
     "da_argmax": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "da_pages_gather_attend": (
         c_int,

@@ -33,6 +33,13 @@ SOURCES = (
     "prefill_attention_f32_split.hip",
     "model_rows.hip",
     "decode_linear.hip",
+    "rotary.hip",
+    "paged_attention.hip",
+    "paged_attention_bf16.hip",
+    "paged_attention_f16.hip",
+    "paged_attention_f32.hip",
+    "paged_attention_bf16_e4m3.hip",
+    "paged_attention_f16_e4m3.hip",
 )
 # packed fp32 VALU ops are switched off for every device compile of this library
 HIPCC_FLAGS = (

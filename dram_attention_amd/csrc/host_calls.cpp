@@ -8,10 +8,14 @@
 // 4-layer model 331 / 218, of which 3 us a launch are the runtime's.
 //
 // A call that finds an operand other than the kernels take it returns None (or false): the
-// caller then goes the general way, which takes or refuses it.
+// caller then goes the general way, which takes or refuses it.  The calls of a batch of sequences
+// (rotate, paged_append, paged_attention) are the only way and refuse it themselves.
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
+#include <ATen/core/grad_mode.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -453,9 +457,385 @@ PyObject *block_tail(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- a batch of sequences in HBM --------------------------------------------------------------
+
+const at::Tensor &plain(PyObject *o, const char *name) {
+  const at::Tensor *t = tensor_of(o);
+  TORCH_CHECK_TYPE(t != nullptr, name, " must be a plain torch.Tensor (got ", Py_TYPE(o)->tp_name, ")");
+  return *t;
+}
+const at::Tensor *plain_or_none(PyObject *o, const char *name) { return o == Py_None ? nullptr : &plain(o, name); }
+
+int float_type(const at::Tensor &t, const char *name) {
+  const int code = dtype_code(t);
+  TORCH_CHECK_TYPE(code >= 0, name, " must be float32, float16 or bfloat16 (got ", t.scalar_type(), ")");
+  return code;
+}
+int page_type(const at::Tensor &pages, const at::Tensor &x) {
+  if (pages.scalar_type() == at::kFloat8_e4m3fn) {
+    TORCH_CHECK_TYPE(x.scalar_type() != at::kFloat, "8-bit pages go with 16-bit queries and keys (got float32)");
+    return DA_E4M3;
+  }
+  TORCH_CHECK_TYPE(pages.scalar_type() == x.scalar_type(), "pages of ", pages.scalar_type(), " do not go with ",
+                   x.scalar_type(), " (the same type, or float8_e4m3fn)");
+  return dtype_code(pages);
+}
+int whole_type(const at::Tensor &t, const char *name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64 (got ",
+                   t.scalar_type(), ")");
+  return t.scalar_type() == at::kLong ? DA_I64 : DA_I32;
+}
+void on_device_of(const at::Tensor &x, std::initializer_list<std::pair<const at::Tensor *, const char *>> others) {
+  for (const auto &o : others)
+    if (o.first)
+      TORCH_CHECK(o.first->device() == x.device(), o.second, " is on ", o.first->device(), ", the rows on ", x.device());
+  TORCH_CHECK(x.is_cuda(), "the operands must live on a GPU: the HIP kernels are the only implementation (got device ",
+              x.device(), ")");
+}
+void not_for_gradients(std::initializer_list<const at::Tensor *> all, const char *what) {
+  if (at::GradMode::is_enabled())
+    for (const at::Tensor *t : all)
+      TORCH_CHECK(!t || !t->requires_grad(), what, " has no gradient: call it under torch.no_grad()");
+}
+// What a call writes into, autograd knows as changed.
+void changed(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+bool dense_rows(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+// Rows as the kernels read them: the last axis dense, and where `vectors` 16-byte aligned.
+at::Tensor rows_of(const at::Tensor &t, bool vectors) {
+  bool fits = dense_rows(t);
+  if (vectors) {
+    fits = fits && aligned(t);
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) fits = fits && stride_of(t, d) * (int64_t)t.element_size() % 16 == 0;
+  }
+  if (fits) return t;
+  const Released others;
+  return t.clone(at::MemoryFormat::Contiguous);
+}
+at::Tensor in_line(const at::Tensor &t) {   // a one-dimensional operand
+  if (t.is_contiguous()) return t;
+  const Released others;
+  return t.contiguous();
+}
+
+// How a call turns channels: frequencies (or none), layout, factor.
+struct Turn {
+  const at::Tensor *freqs;
+  bool half;
+  double factor;
+};
+Turn read_turn(Args &in, int64_t head_dim) {
+  Turn t = {plain_or_none(in.next(), "freqs"), in.integer() != 0, in.number()};
+  TORCH_CHECK_TYPE(in.ok, "factor must be a number");
+  if (t.freqs) {
+    TORCH_CHECK_TYPE(t.freqs->scalar_type() == at::kDouble, "freqs must be float64 (got ", t.freqs->scalar_type(), ")");
+    TORCH_CHECK_VALUE(t.freqs->dim() == 1 && t.freqs->is_contiguous(), "freqs must be one contiguous row");
+    TORCH_CHECK_VALUE(2 * t.freqs->numel() <= head_dim, t.freqs->numel(), " frequencies turn ", 2 * t.freqs->numel(),
+                      " channels, but heads have ", head_dim);
+    TORCH_CHECK_VALUE(t.freqs->numel() <= 256, "up to 256 frequencies (got ", t.freqs->numel(), ")");
+  }
+  return t;
+}
+
+// rotate(xq, xk, positions, freqs, half, factor, inverse, in_place, stream) -> (yq, yk); xk and yk may be None.
+PyObject *rotate(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  Args in{argv, argc};
+  const at::Tensor &xq = plain(in.next(), "xq"), *xk = plain_or_none(in.next(), "xk");
+  const at::Tensor &positions = plain(in.next(), "positions");
+  const int dtype = float_type(xq, "xq");
+  const int64_t dims = xq.dim();
+  TORCH_CHECK_VALUE(dims == 3 || dims == 4, "xq must be (tokens, heads, head_dim) or (batch, tokens, heads, head_dim)");
+  const int64_t D = xq.size(-1), S = xq.size(dims - 3), B = dims == 4 ? xq.size(0) : 1;
+  TORCH_CHECK_VALUE(D > 0, "heads without channels");
+  const Turn turn = read_turn(in, D);
+  TORCH_CHECK_TYPE(turn.freqs != nullptr, "freqs must be a tensor");
+  const bool inverse = in.integer() != 0, in_place = in.integer() != 0;
+  void *stream = in.pointer();
+  TORCH_CHECK_TYPE(in.ok, "rotate: bad argument");
+  if (xk) {
+    TORCH_CHECK_TYPE(xk->scalar_type() == xq.scalar_type(), "xk is ", xk->scalar_type(), " but xq is ", xq.scalar_type());
+    TORCH_CHECK_VALUE(xk->dim() == dims && xk->size(-1) == D && xk->size(dims - 3) == S && (dims == 3 || xk->size(0) == B),
+                      "xk ", xk->sizes(), " does not go with xq ", xq.sizes());
+  }
+  const int position_type = whole_type(positions, "positions");
+  const bool shared = positions.dim() == 1;
+  TORCH_CHECK_VALUE(shared ? positions.size(0) == S : dims == 4 && positions.dim() == 2 && positions.size(0) == B &&
+                                                          positions.size(1) == S,
+                    "positions ", positions.sizes(), " do not go with xq ", xq.sizes());
+  on_device_of(xq, {{xk, "xk"}, {&positions, "positions"}, {turn.freqs, "freqs"}});
+  if (in_place) {
+    not_for_gradients({&xq, xk}, "rotate_");
+    for (const at::Tensor *t : {&xq, xk}) {
+      if (!t) continue;
+      TORCH_CHECK_VALUE(dense_rows(*t) && at::has_internal_overlap(*t) != at::MemOverlap::Yes,
+                        "what is turned in place must have dense rows that do not share memory");
+    }
+    if (xk) {
+      const auto overlap = at::get_overlap_status(xq, *xk);
+      TORCH_CHECK_VALUE(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial,
+                        "xq and xk share memory");
+    }
+  }
+  const c10::DeviceGuard guard(xq.device());
+  const at::Tensor q = in_place ? xq : rows_of(xq, false), k = !xk ? at::Tensor() : in_place ? *xk : rows_of(*xk, false);
+  at::Tensor yq = in_place ? xq : empty_like(xq.sizes(), xq), yk;
+  if (xk) yk = in_place ? *xk : empty_like(xk->sizes(), *xk);
+  da_rotate_args a = {};
+  const int64_t tok = dims - 3;
+  auto strides = [&](const at::Tensor &t, int64_t *to) {
+    to[0] = dims == 4 ? stride_of(t, 0) : 0;
+    to[1] = stride_of(t, tok);
+    to[2] = stride_of(t, tok + 1);
+  };
+  a.q = q.data_ptr();
+  a.q_out = yq.data_ptr();
+  strides(q, a.q_strides);
+  strides(yq, a.q_out_strides);
+  a.n_q_heads = (int32_t)q.size(tok + 1);
+  if (xk) {
+    a.k = k.data_ptr();
+    a.k_out = yk.data_ptr();
+    strides(k, a.k_strides);
+    strides(yk, a.k_out_strides);
+    a.n_k_heads = (int32_t)k.size(tok + 1);
+  }
+  a.freqs = (const double *)turn.freqs->data_ptr();
+  a.positions = positions.data_ptr();
+  a.position_strides[0] = shared ? 0 : stride_of(positions, 0);
+  a.position_strides[1] = stride_of(positions, positions.dim() - 1);
+  a.batch = B;
+  a.tokens = S;
+  a.head_dim = (int32_t)D;
+  a.rotary_dim = (int32_t)(2 * turn.freqs->numel());
+  a.layout = turn.half ? DA_ROTARY_HALF : DA_ROTARY_INTERLEAVED;
+  a.inverse = inverse;
+  a.dtype = dtype;
+  a.position_type = position_type;
+  a.factor = (float)turn.factor;
+  const int rc = unlocked([&] { return da_rotate(&a, sizeof(a), stream); });
+  if (rc) return raise(rc, "da_rotate");
+  if (in_place) {
+    changed(yq);
+    if (xk) changed(yk);
+  }
+  PyObject *second = Py_None;
+  if (xk)
+    second = wrap(std::move(yk));
+  else
+    Py_INCREF(second);
+  return tuple_of({wrap(std::move(yq)), second});
+  END_HANDLE_TH_ERRORS
+}
+
+// What both calls on a paged cache look at: the pools and the table.
+struct Pages {
+  const at::Tensor &k, &v, &table;
+  int type;
+};
+Pages read_pages(Args &in, const at::Tensor &x) {
+  const at::Tensor &k = plain(in.next(), "k_pages"), &v = plain(in.next(), "v_pages"), &table = plain(in.next(), "page_table");
+  TORCH_CHECK_VALUE(k.dim() == 4 && k.sizes() == v.sizes(), "k_pages ", k.sizes(), " and v_pages ", v.sizes(),
+                    " must both be (pages, page_size, kv heads, head_dim)");
+  TORCH_CHECK_TYPE(k.scalar_type() == v.scalar_type(), "k_pages is ", k.scalar_type(), " but v_pages is ", v.scalar_type());
+  const int type = page_type(k, x);
+  TORCH_CHECK_VALUE(k.size(1) > 0 && k.size(2) > 0, "pages without tokens or heads");
+  TORCH_CHECK_VALUE(dense_rows(k) && dense_rows(v), "head_dim must be the dense axis of the pages");
+  for (int64_t d = 0; d < 3; ++d)
+    TORCH_CHECK_VALUE(stride_of(k, d) == stride_of(v, d), "k_pages and v_pages must have the same strides");
+  for (int64_t d = 0; d < 4; ++d) TORCH_CHECK_VALUE(k.size(d) <= 0x7fffffff, "pages ", k.sizes(), " are too many");
+  whole_type(table, "page_table");
+  TORCH_CHECK_VALUE(table.dim() == 2 && dense_rows(table) && table.size(0) <= 0x7fffffff && table.size(1) <= 0x7fffffff,
+                    "page_table must be (sequences, pages) with dense rows");
+  return {k, v, table, type};
+}
+template <typename A>
+void give_pages(A &a, const Pages &p) {
+  for (int d = 0; d < 3; ++d) a.page_strides[d] = stride_of(p.k, d);
+  a.page_table = p.table.data_ptr();
+  a.table_stride = stride_of(p.table, 0);
+  a.table_type = whole_type(p.table, "page_table");
+  a.n_pages = (int32_t)p.k.size(0);
+  a.page_size = (int32_t)p.k.size(1);
+  a.n_sequences = (int32_t)p.table.size(0);
+  a.pages_per_sequence = (int32_t)p.table.size(1);
+  a.n_kv_heads = (int32_t)p.k.size(2);
+  a.head_dim = (int32_t)p.k.size(3);
+  a.page_dtype = p.type;
+}
+const at::Tensor *read_scale(PyObject *o, const char *name, const Pages &p) {
+  const at::Tensor *t = plain_or_none(o, name);
+  if (t) {
+    TORCH_CHECK_VALUE(p.type == DA_E4M3, name, " is for 8-bit pages (these are ", p.k.scalar_type(), ")");
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, name, " must be float32 (got ", t->scalar_type(), ")");
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == p.k.size(2) && t->is_contiguous(), name,
+                      " must hold one number per kv head");
+  }
+  return t;
+}
+const float *numbers(const at::Tensor *t) { return t ? (const float *)t->data_ptr() : nullptr; }
+
+// paged_append(xk, xv, k_pages, v_pages, page_table, positions, sequences, xq, freqs, half, factor, k_scale, v_scale,
+// stream) -> the turned queries, or None without any.
+PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  Args in{argv, argc};
+  const at::Tensor &xk = plain(in.next(), "xk"), &xv = plain(in.next(), "xv");
+  const int dtype = float_type(xk, "xk");
+  const Pages pages = read_pages(in, xk);
+  const at::Tensor &positions = plain(in.next(), "positions"), *sequences = plain_or_none(in.next(), "sequences");
+  const at::Tensor *xq = plain_or_none(in.next(), "xq");
+  const int64_t H = pages.k.size(2), D = pages.k.size(3);
+  const Turn turn = read_turn(in, D);
+  const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
+  void *stream = in.pointer();
+  TORCH_CHECK_TYPE(in.ok, "append_kv_pages_: bad argument");
+  TORCH_CHECK_VALUE(xk.dim() == 3 && xk.size(1) == H && xk.size(2) == D && xv.sizes() == xk.sizes(), "xk ", xk.sizes(),
+                    " and xv ", xv.sizes(), " must both be (tokens, ", H, ", ", D, ") as the pages are");
+  const int64_t T = xk.size(0);
+  TORCH_CHECK_TYPE(xv.scalar_type() == xk.scalar_type(), "xv is ", xv.scalar_type(), " but xk is ", xk.scalar_type());
+  if (xq) {
+    TORCH_CHECK_TYPE(xq->scalar_type() == xk.scalar_type(), "xq is ", xq->scalar_type(), " but xk is ", xk.scalar_type());
+    TORCH_CHECK_VALUE(xq->dim() == 3 && xq->size(0) == T && xq->size(2) == D, "xq ", xq->sizes(), " does not go with xk ",
+                      xk.sizes());
+  }
+  const int position_type = whole_type(positions, "positions");
+  const int sequence_type = sequences ? whole_type(*sequences, "sequences") : DA_I32;
+  TORCH_CHECK_VALUE(positions.dim() == 1 && positions.size(0) == T, "positions ", positions.sizes(), " do not go with ", T,
+                    " tokens");
+  TORCH_CHECK_VALUE(!sequences || (sequences->dim() == 1 && sequences->size(0) == T), "sequences must name one for each of ",
+                    T, " tokens");
+  TORCH_CHECK_VALUE(sequences || T == pages.table.size(0), T, " tokens for the ", pages.table.size(0),
+                    " sequences of the table: say which with sequences=");
+  not_for_gradients({&xk, &xv, xq, &pages.k, &pages.v}, "append_kv_pages_");
+  for (const at::Tensor *t : {&pages.k, &pages.v})
+    TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "pages must not share memory");
+  on_device_of(xk, {{&xv, "xv"}, {&pages.k, "k_pages"}, {&pages.v, "v_pages"}, {&pages.table, "page_table"},
+                    {&positions, "positions"}, {sequences, "sequences"}, {xq, "xq"}, {turn.freqs, "freqs"},
+                    {k_scale, "k_scale"}, {v_scale, "v_scale"}});
+  const c10::DeviceGuard guard(xk.device());
+  const at::Tensor k = rows_of(xk, false), v = rows_of(xv, false), q = xq ? rows_of(*xq, false) : at::Tensor();
+  const at::Tensor at_positions = in_line(positions), of = sequences ? in_line(*sequences) : at::Tensor();
+  at::Tensor out;
+  if (xq) out = empty_like(xq->sizes(), *xq);
+  da_paged_append_args a = {};
+  give_pages(a, pages);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_pages = pages.k.data_ptr();
+  a.v_pages = pages.v.data_ptr();
+  a.positions = at_positions.data_ptr();
+  a.sequences = sequences ? of.data_ptr() : nullptr;
+  a.k_scale = numbers(k_scale);
+  a.v_scale = numbers(v_scale);
+  for (int d = 0; d < 2; ++d) {
+    a.k_strides[d] = stride_of(k, d);
+    a.v_strides[d] = stride_of(v, d);
+    if (xq) {
+      a.q_strides[d] = stride_of(q, d);
+      a.q_out_strides[d] = stride_of(out, d);
+    }
+  }
+  if (xq) {
+    a.q = q.data_ptr();
+    a.q_out = out.data_ptr();
+    a.n_q_heads = (int32_t)q.size(1);
+  }
+  if (turn.freqs) {
+    a.freqs = (const double *)turn.freqs->data_ptr();
+    a.rotary_dim = (int32_t)(2 * turn.freqs->numel());
+  }
+  a.n_tokens = T;
+  a.layout = turn.half ? DA_ROTARY_HALF : DA_ROTARY_INTERLEAVED;
+  a.dtype = dtype;
+  a.position_type = position_type;
+  a.sequence_type = sequence_type;
+  a.factor = (float)turn.factor;
+  const int rc = unlocked([&] { return da_paged_append(&a, sizeof(a), stream); });
+  if (rc) return raise(rc, "da_paged_append");
+  changed(pages.k);
+  changed(pages.v);
+  if (!xq) Py_RETURN_NONE;
+  return wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(xq, k_pages, v_pages, page_table, lengths, scale, k_scale, v_scale, out, lse, stream) -> output; scale,
+// scales, out and lse may be None.
+PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
+  HANDLE_TH_ERRORS
+  Args in{argv, argc};
+  const at::Tensor &xq = plain(in.next(), "xq");
+  const int dtype = float_type(xq, "xq");
+  const Pages pages = read_pages(in, xq);
+  const at::Tensor &lengths = plain(in.next(), "lengths");
+  const int64_t B = pages.table.size(0), H = pages.k.size(2), D = pages.k.size(3);
+  PyObject *scale_at = in.next();
+  double scale = 1.0 / std::sqrt((double)D);
+  if (scale_at != Py_None) {
+    scale = PyFloat_AsDouble(scale_at);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite (got ", scale, ")");
+  }
+  const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
+  const at::Tensor *out_given = plain_or_none(in.next(), "out"), *lse = plain_or_none(in.next(), "lse");
+  void *stream = in.pointer();
+  TORCH_CHECK_TYPE(in.ok, "paged_decode_attention: bad argument");
+  TORCH_CHECK_VALUE(xq.dim() == 3 && xq.size(0) == B && xq.size(2) == D && xq.size(1) > 0 && xq.size(1) % H == 0, "xq ",
+                    xq.sizes(), " must be (", B, " sequences, a multiple of ", H, " heads, ", D, ")");
+  const int64_t Hq = xq.size(1);
+  const int length_type = whole_type(lengths, "lengths");
+  TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == B, "lengths must hold one for each of ", B, " sequences");
+  if (out_given)
+    TORCH_CHECK_VALUE(out_given->sizes() == xq.sizes() && out_given->scalar_type() == xq.scalar_type() &&
+                          out_given->is_contiguous() && aligned(*out_given),
+                      "out must be contiguous, 16-byte aligned and of xq's shape and type");
+  if (lse)
+    TORCH_CHECK_VALUE(lse->scalar_type() == at::kFloat && is_shape(*lse, {B, Hq}) && lse->is_contiguous(),
+                      "lse must be contiguous float32 of shape (sequences, heads)");
+  not_for_gradients({&xq, &pages.k, &pages.v, k_scale, v_scale, out_given}, "paged_decode_attention");
+  on_device_of(xq, {{&pages.k, "k_pages"}, {&pages.v, "v_pages"}, {&pages.table, "page_table"}, {&lengths, "lengths"},
+                    {k_scale, "k_scale"}, {v_scale, "v_scale"}, {out_given, "out"}, {lse, "lse"}});
+  const c10::DeviceGuard guard(xq.device());
+  const at::Tensor q = rows_of(xq, true), lens = in_line(lengths);
+  at::Tensor out = out_given ? *out_given : empty_like(xq.sizes(), xq), room;
+  da_paged_attention_args a = {};
+  give_pages(a, pages);
+  a.q = q.data_ptr();
+  a.k_pages = pages.k.data_ptr();
+  a.v_pages = pages.v.data_ptr();
+  a.lengths = lens.data_ptr();
+  a.k_scale = numbers(k_scale);
+  a.v_scale = numbers(v_scale);
+  a.out = out.data_ptr();
+  a.lse = lse ? (float *)lse->data_ptr() : nullptr;
+  a.q_strides[0] = stride_of(q, 0);
+  a.q_strides[1] = stride_of(q, 1);
+  a.n_q_heads = (int32_t)Hq;
+  a.dtype = dtype;
+  a.length_type = length_type;
+  a.scale = (float)scale;
+  const size_t need = da_paged_attention_workspace_bytes(&a, sizeof(a));
+  if (need) {   // (the call's own: freed at its end, which the caching allocator orders behind the launches)
+    const Released others;
+    room = at::empty({(int64_t)need}, xq.options().dtype(at::kByte).requires_grad(false));
+    a.workspace = room.data_ptr();
+    a.workspace_bytes = (int64_t)need;
+  }
+  const int rc = unlocked([&] { return da_paged_attention(&a, sizeof(a), stream); });
+  if (rc) return raise(rc, "da_paged_attention");
+  if (out_given) changed(out);
+  if (lse) changed(*lse);
+  return wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define DA_CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {DA_CALL(step_args), DA_CALL(static_step), DA_CALL(alike), DA_CALL(linears),
-                         DA_CALL(qkv_rope),  DA_CALL(block_tail),  {nullptr, nullptr, 0, nullptr}};
+                         DA_CALL(qkv_rope),  DA_CALL(block_tail),  DA_CALL(rotate), DA_CALL(paged_append),
+                         DA_CALL(paged_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods};
 
 }  // namespace

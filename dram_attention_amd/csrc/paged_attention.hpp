@@ -1,0 +1,601 @@
+// Attention of one new token of every sequence of a batch over its keys and values in pages:
+//
+//   out[b, j] = sum_t w_t v_t / sum_t w_t,  w_t = exp(q[b, j] . k_t * scale - m),  m = the running maximum
+//
+// Bound: HBM.  Every key and value is read once for all the query heads that share it; a group's query rows are
+// padded to 16 so that both products are 16x16 matrix instructions, which cost next to nothing beside the loads.
+//
+// Split: the sequences of a kv head are laid end to end, in units of kWaves tiles of tokens, and every workgroup takes
+// an equal share of that line, whatever the sequences' lengths: a share may be part of one sequence or hold several.
+// Where the shares begin follows from the lengths, which only the device knows: every workgroup adds them up itself
+// (a block scan of the batch's lengths out of the L2).  A sequence that one share holds whole is finished there; of
+// the others each share leaves its sums, at most two, which paged_join_kernel joins by their maxima.
+//
+// Tile of a wave (16-bit products), 2 sets of 16 tokens, lane l = 16 g + c:
+//   S^T (tokens x rows)  = K Q^T      K rows from global memory are the A operand: lane (g, c) holds token c
+//   O^T (D x rows)      += V^T P^T    the accumulator layout of S^T (lane (g, c): tokens 4g .. 4g+3 of row c) is the
+//                                     B operand as it stands, if the product's k index counts tokens in that order
+// V^T is the A operand: lane (g, c) holds its 8 tokens of one channel.  A lane loads the slice of D/16 channels that is
+// its own of each of its 8 tokens (whole rows per instruction) and pairs the tokens' halves up by byte permutes, 4 a
+// channel, so V needs no LDS.  Weights go in as sums of two 16-bit numbers
+// (split_weights), so that they keep 16 bits: the matrix cores have the room, and the result's error is that of its own
+// rounding.  fp32: tiles of 16 tokens, the same layouts with k = 4, nothing is rounded.
+// e4m3 keys and values become 16-bit ones (exactly) in registers; their heads' scales go into the scores and the output.
+//
+// The K registers are loaded anew as soon as the scores are formed, the V registers as soon as they are consumed, page
+// numbers a tile ahead of both: one set of registers each, always in flight.
+#pragma once
+#include "attention_mfma.hpp"
+#include "paged_math.hpp"
+
+namespace da {
+
+constexpr int kPagedThreads = 256;
+constexpr int kPagedWaves = kPagedThreads / 64;
+
+struct PagedArgs {
+  const char *q, *k, *v;
+  int64_t q_seq_b, q_head_b, page_b, tok_b, head_b;
+  const void *table, *lengths;
+  int64_t table_stride;
+  int32_t table64, lengths64;
+  int32_t n_seqs, n_pages, max_tokens;
+  Divisor by_page;
+  int32_t n_q_heads, n_kv_heads, rep, groups;   // groups: of 16 query rows, of a kv head
+  int32_t shares;                               // 0: a workgroup per sequence, nothing is joined
+  float scale_log2;
+  const float *k_scale, *v_scale;
+  char *out;
+  float *lse;
+  float *part_acc, *part_ml;                    // [head group][share][2][row]
+  int32_t *prefix;                              // units before sequence b; [n_seqs]: all
+};
+
+// How the two products take keys and values of type KV under queries of type T.
+template <typename T, typename KV, int kD>
+struct PagedTile {
+  static constexpr bool kWide = T::kBytes == 4;          // fp32 products
+  static constexpr int kSets = kWide ? 1 : 2;            // of 16 tokens
+  static constexpr int kTokens = 16 * kSets;
+  static constexpr int kUnit = kTokens * kPagedWaves;
+  static constexpr int kSteps = kWide ? kD / 16 : kD / 32;   // 16-byte pieces of a query row a lane holds
+  static constexpr int kSlice = kD / 16;                 // channels of a value row a lane holds
+  static constexpr int kSliceWords = (kSlice * KV::kBytes + 3) / 4;
+  static constexpr int kRowWords = kD * KV::kBytes / 16;     // dwords of a key row a lane holds
+  // a lane's channels: kSlice in a row, but of 96 four out of the first 64 and two out of the others
+  static __device__ __forceinline__ int channel(int r, int j) {
+    if constexpr (kD == 96) return j < 4 ? 4 * r + j : 64 + 2 * r + (j - 4);
+    return kSlice * r + j;
+  }
+  // The first of the (8, or fp32 4) channels that piece s of a query row holds in lane group g.
+  static __device__ __forceinline__ int piece(int s, int g) {
+    if constexpr (kWide) return 16 * s + 4 * g;
+    if constexpr (KV::kBytes == 1) return s / 2 < kD / 64 ? 64 * (s / 2) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g;
+    return 32 * s + 8 * g;
+  }
+};
+
+// log2(e) is in the scores already, so weights are powers of two.  fp16 weights are taken 2^11 times
+// themselves and rescaled early, so that small ones keep their bits: they are 0 below 2^-36 of the largest.
+template <typename T>
+struct WeightRange {
+  static constexpr float kSlack = kRescaleSlack, kBias = 0.f;
+};
+template <>
+struct WeightRange<F16> {
+  static constexpr float kSlack = 4.f, kBias = 11.f;
+};
+
+// Two e4m3 as two elements of T, exactly: the low or high half of w.
+template <typename T, bool kHigh>
+__device__ __forceinline__ uint32_t widen_e4m3(uint32_t w) {
+  if constexpr (__is_same(T, BF16))
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, kHigh));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, kHigh));
+}
+
+// Two weights as the sums of two numbers of T each (dwords).  The first number is below the weight, so that both are
+// positive: an infinite value times them is infinite, where a rest of 0 or less would make NaN of it.  What is left out is
+// at most 2^-15 of a weight (bf16: the rest is at most 2^-7 of it) or 1.5 * 2^-21 (fp16: 1.5 * 2^-10).
+template <typename T>
+__device__ __forceinline__ void split_weights(float lo, float hi, uint32_t &first, uint32_t &rest) {
+  if constexpr (__is_same(T, BF16)) {
+    const uint32_t a = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, lo), 1u);
+    const uint32_t b = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, hi), 1u);
+    first = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    rest = pack_bf16(lo - as_f32(a & 0xffff0000u), hi - as_f32(b & 0xffff0000u));
+  } else {
+    constexpr float kBelow = 1.f - 1.f / 2048;
+    first = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo * kBelow, hi * kBelow));
+    rest = pack_f16(lo - f16_lo(first), hi - f16_hi(first));
+  }
+}
+
+__device__ __forceinline__ int sequence_length(const PagedArgs &a, int b) {
+  const int64_t n = load_index(a.lengths, a.lengths64, b);
+  return n < 0 ? 0 : n < a.max_tokens ? (int)n : a.max_tokens;
+}
+
+// The sums of a row over a stretch of its sequence, or over all of it (`whole`: then the output).
+// `out_row`: b * n_q_heads + query head.
+template <typename T, typename Tile, int kJ>
+__device__ __forceinline__ void write_sums(const PagedArgs &a, bool whole, int64_t out_row, int64_t part_row, int kD,
+                                           int r, int j0, float m, float l, float v_scale, const float *at) {
+  if (whole) {
+    const float by = l > 0.f ? v_scale / l : l == 0.f ? 0.f : l;   // (no token, or NaN)
+    char *o = a.out + out_row * kD * T::kBytes;
+    float f[kJ];
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) f[j] = l == 0.f ? 0.f : at[j] * by;
+    if constexpr (T::kBytes == 2) {
+      uint32_t w[kJ / 2];
+#pragma unroll
+      for (int j = 0; j < kJ / 2; ++j) w[j] = MatrixOps<T>::pack(f[2 * j], f[2 * j + 1]);
+#pragma unroll
+      for (int j = 0; j < kJ / 2; ++j) ((uint32_t *)o)[Tile::channel(r, j0 + 2 * j) / 2] = w[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < kJ; ++j) ((float *)o)[Tile::channel(r, j0 + j)] = f[j];
+    }
+    if (a.lse != nullptr && r == 0 && j0 == 0) a.lse[out_row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  } else {
+    float *p = a.part_acc + part_row * kD;
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) p[Tile::channel(r, j0 + j)] = at[j];
+    if (r == 0 && j0 == 0) {
+      a.part_ml[part_row * 2] = m;
+      a.part_ml[part_row * 2 + 1] = l;
+    }
+  }
+}
+
+template <typename T, typename KV, int kD>
+__global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const PagedArgs a) {
+  using Tile = PagedTile<T, KV, kD>;
+  constexpr bool kWide = Tile::kWide;
+  constexpr int kSets = Tile::kSets, kTokens = Tile::kTokens, kUnit = Tile::kUnit, kSteps = Tile::kSteps;
+  constexpr int kSlice = Tile::kSlice, kSliceWords = Tile::kSliceWords, kRowWords = Tile::kRowWords;
+  constexpr int kHeld = 4 * kSets;                       // tokens whose scores and values a lane holds
+  constexpr int kJ = kSlice > 8 ? 8 : kSlice;            // channels of a slice that are joined at a time
+  constexpr int kRow = 16 * kJ + 4;                      // floats; the pad spreads rows over banks
+  using Range = WeightRange<T>;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+
+  __shared__ int64_t offsets[kPagedWaves][kTokens];
+  __shared__ float sm_m[kPagedWaves][16], sm_l[kPagedWaves][16];
+  __shared__ __align__(16) float sm_acc[kPagedWaves][16][kRow];
+  __shared__ int place[4];
+
+  const int head_groups = a.n_kv_heads * a.groups;
+  const int hg = (int)(blockIdx.x % (unsigned)head_groups), share = (int)(blockIdx.x / (unsigned)head_groups);
+  const int h = hg / a.groups, group = hg - h * a.groups;
+  const int rows = a.rep - 16 * group < 16 ? a.rep - 16 * group : 16;
+  const int64_t first_q = (int64_t)h * a.rep + 16 * group;
+  const float scale_log2 = a.scale_log2 * (KV::kBytes == 1 && a.k_scale ? a.k_scale[h] : 1.f);
+  const float v_scale = KV::kBytes == 1 && a.v_scale ? a.v_scale[h] : 1.f;
+
+  // ---- this workgroup's share: units [u, u_end) of the line, from sequence b that has `before` units ahead of it
+  int b = share, before = 0, u = 0, u_end = 0;
+  if (a.shares == 0) {
+    u_end = (sequence_length(a, b) + kUnit - 1) / kUnit;
+  } else {
+    int total;
+    if (a.n_seqs == 1) {
+      total = (sequence_length(a, 0) + kUnit - 1) / kUnit;
+      b = 0;
+      if (blockIdx.x == 0 && threadIdx.x == 0) a.prefix[0] = 0, a.prefix[1] = total;
+    } else {
+      const int per = (a.n_seqs + kPagedThreads - 1) / kPagedThreads;
+      const int first = (int)threadIdx.x * per, last = min(first + per, a.n_seqs);
+      int sum = 0;
+      for (int i = first; i < last; ++i) sum += (sequence_length(a, i) + kUnit - 1) / kUnit;
+      int upto = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += other;
+      }
+      if (lane == 63) place[wave] = upto;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < kPagedWaves; ++w) {
+        if (w < wave) upto += place[w];
+        total += place[w];
+      }
+      __syncthreads();
+      const int each = (total + a.shares - 1) / a.shares, begin = min(share * each, total);
+      int at = upto - sum;
+      if (blockIdx.x == 0) {
+        for (int i = first, n = at; i < last; ++i) {
+          a.prefix[i] = n;
+          n += (sequence_length(a, i) + kUnit - 1) / kUnit;
+        }
+        if (threadIdx.x == 0) a.prefix[a.n_seqs] = total;
+      }
+      if (at <= begin && begin < upto) {   // one thread, if there is anything to do
+        int i = first;
+        for (; i < last - 1; ++i) {
+          const int n = (sequence_length(a, i) + kUnit - 1) / kUnit;
+          if (at + n > begin) break;
+          at += n;
+        }
+        place[0] = i, place[1] = at;
+      }
+      __syncthreads();
+      b = place[0], before = place[1];
+    }
+    const int each = (total + a.shares - 1) / a.shares;
+    u = min(share * each, total), u_end = min(u + each, total);
+    // sequences without tokens, one after the other to the shares
+    for (int i = share; i < a.n_seqs; i += a.shares) {
+      if (sequence_length(a, i) > 0) continue;
+      for (int x = threadIdx.x; x < rows * kD; x += kPagedThreads) {
+        const int64_t row = (int64_t)i * a.n_q_heads + first_q + x / kD;
+        store_elem<T>(a.out, row * kD + x % kD, 0.f);
+        if (a.lse != nullptr && x % kD == 0) a.lse[row] = -INFINITY;
+      }
+    }
+  }
+  if (a.shares == 0 && u_end == 0) {
+    for (int x = threadIdx.x; x < rows * kD; x += kPagedThreads) {
+      const int64_t row = (int64_t)b * a.n_q_heads + first_q + x / kD;
+      store_elem<T>(a.out, row * kD + x % kD, 0.f);
+      if (a.lse != nullptr && x % kD == 0) a.lse[row] = -INFINITY;
+    }
+  }
+
+  const char *kbase = a.k + h * a.head_b, *vbase = a.v + h * a.head_b;
+  // (b stays in range even if a length changes while this runs)
+  for (; u < u_end && b < a.n_seqs; ++b) {
+    const int len = sequence_length(a, b), units = (len + kUnit - 1) / kUnit;
+    if (units == 0) continue;
+    const int from = u - before, to = min(u_end - before, units);
+    const int t0 = from * kUnit, t1 = min(to * kUnit, len);
+    const bool whole = from == 0 && to == units;
+    const int64_t table_row = b * a.table_stride;
+
+    u32x4 qv[kSteps];
+    {
+      const char *qp = a.q + b * a.q_seq_b + (first_q + (c < rows ? c : 0)) * a.q_head_b;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        qv[s] = load16(qp + Tile::piece(s, g) * T::kBytes);
+        if (c >= rows) qv[s] = u32x4{0, 0, 0, 0};
+      }
+    }
+
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc[kSlice];
+#pragma unroll
+    for (int j = 0; j < kSlice; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    uint32_t kk[kSets][kRowWords];
+    uint32_t vv[kHeld][kSliceWords];
+    uint32_t live = 0;   // of the tokens held: which count
+
+    // The page number of the lane's token of a tile (any valid table entry past the end).
+    auto page_of = [&](int tile) {
+      const int t = min(tile + (lane & (kTokens - 1)), t1 - 1);
+      return load_index(a.table, a.table64, table_row + divide(t, a.by_page));
+    };
+    // Byte offsets of the tile's tokens in the pool, -1 for those that do not count, for the wave's lanes to read.
+    auto publish = [&](int tile, int64_t page) {
+      const int t = tile + (lane & (kTokens - 1)), slot = t - divide(min(t, t1 - 1), a.by_page) * a.by_page.d;
+      const bool counts = t < t1 && page >= 0 && page < a.n_pages;
+      if (lane < kTokens) offsets[wave][lane] = counts ? page * a.page_b + (int64_t)slot * a.tok_b : -1;
+      __builtin_amdgcn_wave_barrier();
+    };
+    auto load_keys = [&]() {
+#pragma unroll
+      for (int s = 0; s < kSets; ++s) {
+        const int64_t off = offsets[wave][16 * s + c];
+        const char *p = kbase + (off < 0 ? 0 : off);
+#pragma unroll
+        for (int w = 0; w + 4 <= kRowWords; w += 4) {
+          const u32x4 x = load16(p + (w * 4 + g * 4) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) kk[s][w + i] = x[i];
+        }
+        if constexpr (kRowWords % 4 == 2) {   // (96 e4m3)
+          const u32x2 x = *(const u32x2 *)(p + (kRowWords - 2) * 16 + g * 8);
+          kk[s][kRowWords - 2] = x[0], kk[s][kRowWords - 1] = x[1];
+        }
+      }
+    };
+    auto load_values = [&]() {
+      live = 0;
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x) {
+        const int64_t off = offsets[wave][16 * (x / 4) + 4 * g + x % 4];
+        live |= (off < 0 ? 0u : 1u) << x;
+        const char *p = vbase + (off < 0 ? 0 : off);
+        if constexpr (kD == 96) {
+          if constexpr (KV::kBytes == 1) {
+            vv[x][0] = *(const uint32_t *)(p + 4 * c);
+            vv[x][1] = *(const uint16_t *)(p + 64 + 2 * c);
+          } else if constexpr (KV::kBytes == 2) {
+            const u32x2 y = *(const u32x2 *)(p + 8 * c);
+            vv[x][0] = y[0], vv[x][1] = y[1];
+            vv[x][2] = *(const uint32_t *)(p + 128 + 4 * c);
+          } else {
+            const u32x4 y = load16(p + 16 * c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vv[x][i] = y[i];
+            const u32x2 z = *(const u32x2 *)(p + 256 + 8 * c);
+            vv[x][4] = z[0], vv[x][5] = z[1];
+          }
+        } else if constexpr (kSliceWords == 1) {
+          vv[x][0] = *(const uint32_t *)(p + 4 * c);
+        } else if constexpr (kSliceWords == 2) {
+          const u32x2 y = *(const u32x2 *)(p + 8 * c);
+          vv[x][0] = y[0], vv[x][1] = y[1];
+        } else {
+#pragma unroll
+          for (int w = 0; w < kSliceWords; w += 4) {
+            const u32x4 y = load16(p + (kSliceWords * c + w) * 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vv[x][w + i] = y[i];
+          }
+        }
+      }
+    };
+
+    // S^T of the tile in kk
+    auto scores = [&](f32x4 *st) {
+#pragma unroll
+      for (int s = 0; s < kSets; ++s) {
+        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+        if constexpr (kWide) {
+#pragma unroll
+          for (int i = 0; i < 4 * kSteps; ++i) {   // two chains
+            f32x4 &z = i & 1 ? y : x;
+            z = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(kk[s][i]), as_f32(qv[i / 4][i % 4]), z, 0, 0, 0);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            u32x4 ka;
+            if constexpr (KV::kBytes == 1) {
+              const uint32_t w0 = kk[s][2 * i], w1 = kk[s][2 * i + 1];
+              ka = u32x4{widen_e4m3<T, false>(w0), widen_e4m3<T, true>(w0), widen_e4m3<T, false>(w1),
+                         widen_e4m3<T, true>(w1)};
+            } else {
+              ka = u32x4{kk[s][4 * i], kk[s][4 * i + 1], kk[s][4 * i + 2], kk[s][4 * i + 3]};
+            }
+            f32x4 &z = i & 1 ? y : x;
+            z = MatrixOps<T>::k32(ka, qv[i], z);
+          }
+        }
+        st[s] = x + y;
+      }
+    };
+
+    // Weights of the tile's scores; O^T += V^T P^T
+    auto weigh = [&](const f32x4 *st) {
+      float p[kHeld];
+      float top = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x) {
+        p[x] = live >> x & 1 ? st[x / 4][x % 4] * scale_log2 : -INFINITY;
+        top = fmaxf(top, p[x]);
+      }
+      if (__any(top > m + (Range::kSlack + Range::kBias))) {   // rare
+        float mx = top - Range::kBias;
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
+        const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
+        m = mx;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < kSlice; ++j) acc[j] *= alpha;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x) {
+        p[x] = fast_exp2(p[x] - ref);
+        l += p[x];
+      }
+      // values of tokens that do not count are memory nobody vouches for: 0 * NaN must not arise
+      if (__any(live != (1u << kHeld) - 1)) {
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x)
+#pragma unroll
+          for (int w = 0; w < kSliceWords; ++w) vv[x][w] = live >> x & 1 ? vv[x][w] : 0u;
+      }
+      if constexpr (kWide) {
+#pragma unroll
+        for (int x = 0; x < kHeld; ++x)
+#pragma unroll
+          for (int j = 0; j < kSlice; ++j)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[x], acc[j], 0, 0, 0);
+      } else {
+        u32x4 p1, p2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t first, rest;
+          split_weights<T>(p[2 * i], p[2 * i + 1], first, rest);
+          p1[i] = first, p2[i] = rest;
+        }
+#pragma unroll
+        for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
+          uint32_t w[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            if constexpr (KV::kBytes == 1)
+              w[x] = jj & 1 ? widen_e4m3<T, true>(vv[x][jj / 2]) : widen_e4m3<T, false>(vv[x][jj / 2]);
+            else
+              w[x] = vv[x][jj];
+          }
+          u32x4 even, odd;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+            odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+          }
+          acc[2 * jj] = MatrixOps<T>::k32(even, p1, acc[2 * jj]);
+          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p1, acc[2 * jj + 1]);
+          acc[2 * jj] = MatrixOps<T>::k32(even, p2, acc[2 * jj]);
+          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p2, acc[2 * jj + 1]);
+        }
+      }
+    };
+
+    int tile = t0 + wave * kTokens;
+    if (tile < t1) {
+      int64_t page = page_of(tile), next = page_of(tile + kUnit);
+      publish(tile, page);
+      load_keys();
+      load_values();
+      for (; tile < t1; tile += kUnit) {
+        f32x4 st[kSets];
+        page = page_of(tile + 2 * kUnit);
+        scores(st);
+        publish(tile + kUnit, next);
+        load_keys();
+        weigh(st);
+        load_values();
+        next = page;
+      }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // ---- the waves' sums together
+    const int64_t part = (((int64_t)hg * a.shares + share) * 2 + (from == 0 ? 1 : 0)) * 16;
+#pragma unroll
+    for (int j0 = 0; j0 < kSlice; j0 += kJ) {
+      __syncthreads();   // (what the last pass or sequence left there has been read)
+      if (c < rows) {
+        if (g == 0) sm_m[wave][c] = m, sm_l[wave][c] = l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) sm_acc[wave][c][(4 * g + i) * kJ + j] = acc[j0 + j][i];
+      }
+      __syncthreads();
+      const int row = threadIdx.x >> 4, r = threadIdx.x & 15;
+      if (row < rows) {
+        float mx = sm_m[0][row];
+#pragma unroll
+        for (int w = 1; w < kPagedWaves; ++w) mx = fmaxf(mx, sm_m[w][row]);
+        float sum = 0.f, at[kJ];
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) at[j] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; ++w) {
+          const float by = mx == -INFINITY ? 1.f : fast_exp2(sm_m[w][row] - mx);
+          sum += sm_l[w][row] * by;
+#pragma unroll
+          for (int j = 0; j < kJ; ++j) at[j] += sm_acc[w][row][r * kJ + j] * by;
+        }
+        write_sums<T, Tile, kJ>(a, whole, (int64_t)b * a.n_q_heads + first_q + row, part + row, kD, r, j0, mx, sum,
+                                v_scale, at);
+      }
+    }
+    u = before + to;
+    before += units;
+  }
+}
+
+// The sums of sequences that more than one share holds: a workgroup for each query head and sequence or, where
+// there are fewer, inner border of two shares (the first one inside a sequence finds it).
+template <typename T, int kD>
+__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedArgs a, const bool by_border) {
+  constexpr int kLanes = kD / 4, kParts = kPagedThreads / kLanes;
+  __shared__ __align__(16) float sums[kParts][kD];
+  __shared__ float red[kPagedWaves], ls[kParts];
+  const int hq = (int)(blockIdx.x % (unsigned)a.n_q_heads), at = (int)(blockIdx.x / (unsigned)a.n_q_heads);
+  const int total = a.prefix[a.n_seqs];
+  const int each = (total + a.shares - 1) / a.shares;
+  int b = at;
+  if (by_border) {
+    const int border = (at + 1) * each;
+    if (border >= total) return;
+    int lo = 0, hi = a.n_seqs;   // prefix[lo] <= border < prefix[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.prefix[mid] <= border) lo = mid; else hi = mid;
+    }
+    b = lo;
+    if (a.prefix[b] == border || a.prefix[b] < border - each) return;
+  }
+  const int begin = a.prefix[b], end = a.prefix[b + 1];
+  if (begin == end) return;
+  const int s0 = begin / each, n = (end - 1) / each - s0 + 1;
+  if (n == 1) return;
+  const int h = hq / a.rep, rr = hq - h * a.rep;
+  const int64_t hg = (int64_t)h * a.groups + rr / 16;
+  auto row = [&](int i) { return ((hg * a.shares + s0 + i) * 2 + (i == 0 ? 1 : 0)) * 16 + rr % 16; };
+
+  float mx = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += kPagedThreads) mx = fmaxf(mx, a.part_ml[row(i) * 2]);
+  mx = group_max<64>(mx);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
+  __syncthreads();
+  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+
+  const int part = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  float l = 0.f;
+  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (part < kParts) {
+    for (int i = part; i < n; i += kParts) {
+      const int64_t x = row(i);
+      const float m = a.part_ml[x * 2];
+      const float by = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
+      l += a.part_ml[x * 2 + 1] * by;
+      sum += *(const f32x4 *)(a.part_acc + x * kD + d) * by;
+    }
+    *(f32x4 *)&sums[part][d] = sum;
+  }
+  if (part < kParts && d == 0) ls[part] = l;   // (the same in every lane of a part)
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kParts; ++i) l += ls[i];
+  const int64_t out_row = (int64_t)b * a.n_q_heads + hq;
+  const float v_scale = a.v_scale ? a.v_scale[h] : 1.f;
+  for (int x = threadIdx.x; x < kD; x += kPagedThreads) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) t += sums[i][x];
+    store_elem<T>(a.out, out_row * kD + x, l == 0.f ? 0.f : t * (v_scale / l));
+  }
+  if (threadIdx.x == 0 && a.lse != nullptr) a.lse[out_row] = l == 0.f ? -INFINITY : mx * kLn2 + logf(l);
+}
+
+// Defined per pair of types in paged_attention_*.hip.
+template <typename T, typename KV>
+int launch_paged(const PagedArgs &a, int head_dim, hipStream_t s);
+template <> int launch_paged<BF16, BF16>(const PagedArgs &, int, hipStream_t);
+template <> int launch_paged<F16, F16>(const PagedArgs &, int, hipStream_t);
+template <> int launch_paged<F32, F32>(const PagedArgs &, int, hipStream_t);
+template <> int launch_paged<BF16, E4M3>(const PagedArgs &, int, hipStream_t);
+template <> int launch_paged<F16, E4M3>(const PagedArgs &, int, hipStream_t);
+
+template <typename T, typename KV, int kD>
+int launch_paged_dim(const PagedArgs &a, hipStream_t s) {
+  const unsigned head_groups = (unsigned)(a.n_kv_heads * a.groups);
+  const unsigned blocks = head_groups * (unsigned)(a.shares == 0 ? a.n_seqs : a.shares);
+  hipLaunchKernelGGL((paged_attention_kernel<T, KV, kD>), dim3(blocks), dim3(kPagedThreads), 0, s, a);
+  if (a.shares > 1) {
+    const bool by_border = a.shares - 1 < a.n_seqs;
+    const unsigned joins = (unsigned)a.n_q_heads * (unsigned)(by_border ? a.shares - 1 : a.n_seqs);
+    hipLaunchKernelGGL((paged_join_kernel<T, kD>), dim3(joins), dim3(kPagedThreads), 0, s, a, by_border);
+  }
+  return launch_status("da_paged_attention");
+}
+
+#define DA_PAGED_TYPES(T, KV)                                                         \
+  template <>                                                                         \
+  int launch_paged<T, KV>(const PagedArgs &a, int head_dim, hipStream_t s) {          \
+    switch (head_dim) {                                                               \
+      case 64: return launch_paged_dim<T, KV, 64>(a, s);                              \
+      case 96: return launch_paged_dim<T, KV, 96>(a, s);                              \
+      case 128: return launch_paged_dim<T, KV, 128>(a, s);                            \
+      default: return launch_paged_dim<T, KV, 256>(a, s);                             \
+    }                                                                                 \
+  }
+
+}  // namespace da

@@ -1,0 +1,352 @@
+// Rotary positions: queries and keys turned by their tokens' positions, as tensors of their own (da_rotate,
+// forward and backward) or on the way into the pages of a cache (da_paged_append).
+//
+//   y[a_i] = f (x[a_i] cos t - x[b_i] sin t),  y[b_i] = f (x[a_i] sin t + x[b_i] cos t),  t = position * freqs[i]
+//
+// for the pairs i of a head's first `rotary_dim` channels: (2i, 2i + 1) or (i, i + rotary_dim / 2).  The other
+// channels are copied.  The turn's transpose is the turn by -t: the backward pass is the same kernel.
+//
+// Angles are formed here, in 64 bits, from a position and a frequency: a table of cosines would take 64 MiB per
+// 131072 positions of a head of 128, and angles multiplied out in 32 bits are off by 2^-24 of themselves, 0.06 rad at
+// the millionth position of the fastest pair.  Whole turns go away in 64 bits, then quarters of a turn, and sine and
+// cosine of the rest are Taylor polynomials on |t| <= pi/4 (their next terms are below 2^-26).
+//
+// Bound: HBM; a row is read once and written once, 16 bytes a lane.  A wave takes one token and as many head rows
+// as make kPasses loads of 16 bytes a lane, all in flight while the lanes compute the token's angles, one pair
+// each, into LDS that only this wave reads: no barrier.  A token of many heads is several waves', which form its
+// angles again: they are 40 instructions a pair, and few tokens want many waves.
+#include "paged_math.hpp"
+
+namespace da {
+
+constexpr int kTurnThreads = 256;
+constexpr int kTurnWaves = kTurnThreads / 64;
+constexpr int kMaxPairs = 256;   // rotary_dim / 2
+constexpr int kPasses = 4;
+
+// Head rows: of q, then of k, then (append) of v.
+struct TurnArgs {
+  const char *x[3];
+  char *y[3];
+  int64_t x_batch_b[3], x_tok_b[3], x_head_b[3];
+  int64_t y_batch_b[3], y_tok_b[3], y_head_b[3];   // (y of k and v in pages: page, token, head)
+  int32_t row_end[3];                              // head rows up to and with q's, k's, v's
+  int32_t cols, lanes_shift;                       // items of a row; lanes that take them, as a power of two
+  int32_t head_dim, rotary_dim, half;
+  int32_t windows, waves;                          // waves of a token, of all tokens
+  Divisor by_windows, by_tokens;                   // by_tokens: tokens of a batch
+  const double *freqs;
+  const void *positions;
+  int64_t pos_batch_stride, pos_tok_stride;
+  int32_t positions64;
+  float factor, sign;
+  // append
+  const void *table, *sequences;
+  int64_t table_stride;
+  int32_t table64, sequences64, n_sequences, n_pages, max_tokens;
+  Divisor by_page;
+  const float *scale[3];                           // per kv head, or null
+};
+
+__device__ __forceinline__ void turn_of(double position, double freq, float factor, float sign, float &c, float &s) {
+  double a = position * freq * 0.15915494309189535;   // turns
+  a -= rint(a);
+  const double quarter = rint(4.0 * a);                // -2 .. 2
+  const float t = (float)((a - 0.25 * quarter) * 6.283185307179586);
+  const float u = t * t;
+  float sn = fmaf(u, fmaf(u, fmaf(u, fmaf(u, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), 0.f);
+  sn = fmaf(t, sn, t);
+  float cs = fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f);
+  cs = fmaf(u, cs, 1.f);
+  const int n = (int)quarter & 3;
+  const float c1 = n & 1 ? -sn : cs, s1 = n & 1 ? cs : sn;
+  c = factor * (n & 2 ? -c1 : c1);
+  s = factor * sign * (n & 2 ? -s1 : s1);
+}
+
+template <typename T, int kN>
+__device__ __forceinline__ void load_row(const char *p, int at, float *f) {
+  if constexpr (kN == 1)
+    f[0] = load_elem<T>(p, at);
+  else
+    unpack<T>(load16(p + (int64_t)at * T::kBytes), f);
+}
+// kN values into elements of type TC; e4m3 ones divided by the head's scale first.
+template <typename TC, int kN>
+__device__ __forceinline__ void store_row(char *p, int at, float *f, float scale) {
+  if constexpr (TC::kBytes == 1) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) f[i] = f[i] / scale;
+    if constexpr (kN == 8) {
+      uint32_t *d = (uint32_t *)(p + at);
+      *(uint2 *)d = make_uint2(pack_e4m3(f), pack_e4m3(f + 4));
+    } else {
+      const float one[4] = {f[0], 0.f, 0.f, 0.f};
+      p[at] = (char)pack_e4m3(one);
+    }
+  } else if constexpr (kN == 1) {
+    store_elem<TC>(p, at, f[0]);
+  } else {
+    store16(p + (int64_t)at * TC::kBytes, pack_vec<TC>(f));
+  }
+}
+
+// kN: elements a load (a 16-byte vector, or 1 where a row's parts are no whole vectors).  kPairsInside: the
+// interleaved layout by vectors, whose pairs lie inside one; otherwise an item is the two vectors (or elements) of
+// kN pairs, and behind those single ones that are copied.
+template <typename T, typename TC, int kN, bool kPairsInside, bool kPaged>
+__global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArgs a) {
+  __shared__ float2 turns[kTurnWaves][kMaxPairs];
+  const int lane = threadIdx.x & 63;
+  const int wave = (int)(blockIdx.x * kTurnWaves + (threadIdx.x >> 6));
+  if (wave >= a.waves) return;
+  const int tok = divide(wave, a.by_windows), window = wave - tok * a.windows;
+  const int64_t batch = divide(tok, a.by_tokens), in_batch = tok - (int)batch * a.by_tokens.d;
+  const int64_t pos = load_index(a.positions, a.positions64, batch * a.pos_batch_stride + in_batch * a.pos_tok_stride);
+  const int pairs = a.rotary_dim / 2;
+
+  const int lanes = 1 << a.lanes_shift, rows_per_pass = 64 >> a.lanes_shift;
+  const int first_row = window * rows_per_pass * kPasses + (lane >> a.lanes_shift);
+  const int rows = a.row_end[kPaged ? 2 : 1];
+  const int turned_cols = kPairsInside ? a.rotary_dim / kN : pairs / kN;
+  const int col0 = lane & (lanes - 1);
+
+  auto which = [&](int row) { return row < a.row_end[0] ? 0 : !kPaged || row < a.row_end[1] ? 1 : 2; };
+  // An item's first element, and the second part's (pairs that lie apart).
+  auto at_a = [&](int col) {
+    if (kPairsInside) return col * kN;
+    if (col >= turned_cols) return a.rotary_dim + (col - turned_cols) * kN;
+    return a.half ? col * kN : 2 * col;
+  };
+  auto at_b = [&](int col) { return a.half ? pairs + col * kN : 2 * col + 1; };
+
+  // where the token's keys and values go
+  int64_t page_off = 0;
+  bool stored = true;
+  if constexpr (kPaged) {
+    const int64_t seq = a.sequences ? load_index(a.sequences, a.sequences64, tok) : tok;
+    stored = seq >= 0 && seq < a.n_sequences && pos >= 0 && pos < a.max_tokens;
+    const int at = stored ? (int)pos : 0;
+    const int page = divide(at, a.by_page);
+    const int64_t number = stored ? load_index(a.table, a.table64, seq * a.table_stride + page) : -1;
+    stored = number >= 0 && number < a.n_pages;
+    page_off = (stored ? number : 0) * a.y_batch_b[1] + (int64_t)(at - page * a.by_page.d) * a.y_tok_b[1];
+  }
+
+  // Rows wider than 64 items go in steps of 64.  (Lanes without an item stay: they have angles to form.)
+  for (int base = 0; base < a.cols; base += lanes) {
+    const int col = base + col0, end_row = col < a.cols ? rows : 0;
+    float fa[kPasses][kN], fb[kPasses][kN];
+    const bool paired = !kPairsInside && col < turned_cols;
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+      const int row = first_row + u * rows_per_pass;
+      if (row >= end_row) continue;
+      const int w = which(row), head = row - (w ? a.row_end[w - 1] : 0);
+      const char *p = a.x[w] + batch * a.x_batch_b[w] + in_batch * a.x_tok_b[w] + head * a.x_head_b[w];
+      load_row<T, kN>(p, at_a(col), fa[u]);
+      if (paired) load_row<T, kN>(p, at_b(col), fb[u]);
+    }
+    if (base == 0) {
+      float2 *mine = turns[threadIdx.x >> 6];
+      for (int i = lane; i < pairs; i += 64) {
+        float c, s;
+        turn_of((double)pos, a.freqs[i], a.factor, a.sign, c, s);
+        mine[i] = make_float2(c, s);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+    const float2 *turn = turns[threadIdx.x >> 6];
+    float2 cs[kN];
+    if (col < turned_cols) {
+      constexpr int kPairs = kPairsInside ? kN / 2 : kN;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) cs[i] = turn[col * kPairs + i];
+    }
+#pragma unroll
+    for (int u = 0; u < kPasses; ++u) {
+      const int row = first_row + u * rows_per_pass;
+      if (row >= end_row) continue;
+      const int w = which(row), head = row - (w ? a.row_end[w - 1] : 0);
+      if (col < turned_cols && w < 2) {
+        if constexpr (kPairsInside) {
+#pragma unroll
+          for (int i = 0; i < kN; i += 2) rotate_pair(fa[u][i], fa[u][i + 1], cs[i / 2].x, cs[i / 2].y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) rotate_pair(fa[u][i], fb[u][i], cs[i].x, cs[i].y);
+        }
+      }
+      if (!kPaged || w == 0) {
+        char *d = a.y[w] + batch * a.y_batch_b[w] + in_batch * a.y_tok_b[w] + head * a.y_head_b[w];
+        store_row<T, kN>(d, at_a(col), fa[u], 1.f);
+        if (paired) store_row<T, kN>(d, at_b(col), fb[u], 1.f);
+      } else if (stored) {
+        char *d = a.y[w] + page_off + head * a.y_head_b[w];
+        const float scale = TC::kBytes == 1 && a.scale[w] ? a.scale[w][head] : 1.f;
+        store_row<TC, kN>(d, at_a(col), fa[u], scale);
+        if (paired) store_row<TC, kN>(d, at_b(col), fb[u], scale);
+      }
+    }
+  }
+}
+
+static bool multiple(int64_t v, int of) { return v % of == 0; }
+
+// Fills what follows from the shape; rows of whole 16-byte vectors (`vectors`) or element by element.
+static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool vectors, const char *what) {
+  const int n = vectors ? vec : 1;
+  const bool inside = vectors && !a.half;
+  a.cols = inside ? a.head_dim / n : a.rotary_dim / 2 / n + (a.head_dim - a.rotary_dim) / n;
+  a.lanes_shift = 0;
+  while (a.lanes_shift < 6 && (1 << a.lanes_shift) < a.cols) ++a.lanes_shift;
+  const int rows = a.row_end[2];
+  a.windows = (int)ceil_div(rows, (64 >> a.lanes_shift) * kPasses);
+  // (what is counted in 32 bits; with a few spare waves of the last workgroup)
+  const int64_t most = 0x7fffff00;
+  if (tokens > most / batch || batch * tokens > most / a.windows)
+    return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens, %d waves each, are too many", what, (long long)batch,
+                (long long)tokens, a.windows);
+  a.waves = (int32_t)(batch * tokens * a.windows);
+  a.by_windows = divisor_of(a.windows), a.by_tokens = divisor_of((int32_t)tokens);
+  return DA_OK;
+}
+
+template <typename T, typename TC, bool kPaged>
+static int launch_rows(const TurnArgs &a, bool vectors, hipStream_t s, const char *what) {
+  const dim3 grid((unsigned)ceil_div(a.waves, kTurnWaves)), block(kTurnThreads);
+  if (!vectors)
+    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, 1, false, kPaged>), grid, block, 0, s, a);
+  else if (a.half)
+    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, T::kVec, false, kPaged>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, T::kVec, true, kPaged>), grid, block, 0, s, a);
+  return launch_status(what);
+}
+
+static int check_turn(int head_dim, int rotary_dim, int layout, int dtype, const void *freqs, const char *what) {
+  DA_REQUIRE(dtype == DA_F32 || dtype == DA_F16 || dtype == DA_BF16, "%s: unknown dtype %d", what, dtype);
+  DA_REQUIRE(head_dim > 0 && rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+             "%s: %d channels of %d cannot turn in pairs", what, rotary_dim, head_dim);
+  DA_REQUIRE(layout == DA_ROTARY_INTERLEAVED || layout == DA_ROTARY_HALF, "%s: unknown layout %d", what, layout);
+  DA_REQUIRE(freqs || rotary_dim == 0, "%s: null pointer", what);
+  if (rotary_dim / 2 > kMaxPairs || head_dim > 65536)
+    return fail(DA_ENOTSUP, "%s: up to %d channels that turn, heads of up to 65536", what, 2 * kMaxPairs);
+  return DA_OK;
+}
+// Whether a turned row's parts are whole vectors of `vec` elements.
+static bool whole_vectors(int head_dim, int rotary_dim, int half, int vec) {
+  return multiple(head_dim, vec) && multiple(half ? rotary_dim / 2 : rotary_dim, vec);
+}
+
+}  // namespace da
+
+extern "C" int da_rotate(const void *args, size_t args_bytes, void *stream) {
+  using namespace da;
+  DA_REQUIRE(args && args_bytes == sizeof(da_rotate_args), "da_rotate: an argument block of %d bytes",
+             (int)sizeof(da_rotate_args));
+  da_rotate_args r;
+  memcpy(&r, args, sizeof(r));
+  if (int rc = check_turn(r.head_dim, r.rotary_dim, r.layout, r.dtype, r.freqs, "da_rotate")) return rc;
+  DA_REQUIRE(r.batch >= 0 && r.tokens >= 0 && r.n_q_heads >= 0 && r.n_k_heads >= 0 && r.n_q_heads <= 1 << 20 &&
+                 r.n_k_heads <= 1 << 20,
+             "da_rotate: bad shape");
+  DA_REQUIRE(r.position_type == DA_I32 || r.position_type == DA_I64, "da_rotate: unknown position type %d",
+             r.position_type);
+  if (r.batch == 0 || r.tokens == 0 || r.n_q_heads + r.n_k_heads == 0) return DA_OK;
+  DA_REQUIRE(r.positions && (!r.n_q_heads || (r.q && r.q_out)) && (!r.n_k_heads || (r.k && r.k_out)),
+             "da_rotate: null pointer");
+  const int e = elem_size(r.dtype), vec = 16 / e;
+  TurnArgs a = {};
+  const void *x[2] = {r.q, r.k};
+  void *y[2] = {r.q_out, r.k_out};
+  const int64_t *xs[2] = {r.q_strides, r.k_strides}, *ys[2] = {r.q_out_strides, r.k_out_strides};
+  const int32_t heads[2] = {r.n_q_heads, r.n_k_heads};
+  bool vectors = whole_vectors(r.head_dim, r.rotary_dim, r.layout, vec);
+  for (int i = 0; i < 2; ++i) {
+    a.x[i] = (const char *)x[i];
+    a.y[i] = (char *)y[i];
+    a.x_batch_b[i] = xs[i][0] * e, a.x_tok_b[i] = xs[i][1] * e, a.x_head_b[i] = xs[i][2] * e;
+    a.y_batch_b[i] = ys[i][0] * e, a.y_tok_b[i] = ys[i][1] * e, a.y_head_b[i] = ys[i][2] * e;
+    if (!heads[i]) continue;
+    vectors = vectors && multiple((uintptr_t)x[i] | (uintptr_t)y[i], 16);
+    for (int j = 0; j < 3; ++j) vectors = vectors && multiple(xs[i][j], vec) && multiple(ys[i][j], vec);
+  }
+  a.row_end[0] = r.n_q_heads, a.row_end[1] = a.row_end[2] = r.n_q_heads + r.n_k_heads;
+  a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
+  a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type;
+  a.pos_batch_stride = r.position_strides[0], a.pos_tok_stride = r.position_strides[1];
+  a.factor = r.factor, a.sign = r.inverse ? -1.f : 1.f;
+  if (int rc = shape_rows(a, r.batch, r.tokens, vec, vectors, "da_rotate")) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, false>(a, vectors, s, "da_rotate");
+  if (r.dtype == DA_F16) return launch_rows<F16, F16, false>(a, vectors, s, "da_rotate");
+  return launch_rows<F32, F32, false>(a, vectors, s, "da_rotate");
+}
+
+extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream) {
+  using namespace da;
+  DA_REQUIRE(args && args_bytes == sizeof(da_paged_append_args), "da_paged_append: an argument block of %d bytes",
+             (int)sizeof(da_paged_append_args));
+  da_paged_append_args r;
+  memcpy(&r, args, sizeof(r));
+  if (int rc = check_turn(r.head_dim, r.rotary_dim, r.layout, r.dtype, r.freqs, "da_paged_append")) return rc;
+  DA_REQUIRE(r.page_dtype == r.dtype || r.page_dtype == DA_E4M3, "da_paged_append: pages of type %d for rows of type %d",
+             r.page_dtype, r.dtype);
+  if (r.page_dtype == DA_E4M3 && r.dtype == DA_F32)
+    return fail(DA_ENOTSUP, "da_paged_append: 8-bit pages take 16-bit rows");
+  DA_REQUIRE(r.n_tokens >= 0 && r.n_q_heads >= 0 && r.n_kv_heads > 0 && r.n_q_heads <= 1 << 20 && r.n_kv_heads <= 1 << 20 &&
+                 r.n_sequences >= 0 && r.pages_per_sequence >= 0 && r.page_size > 0 && r.n_pages >= 0,
+             "da_paged_append: bad shape");
+  for (int t : {r.table_type, r.position_type, r.sequence_type})
+    DA_REQUIRE(t == DA_I32 || t == DA_I64, "da_paged_append: unknown integer type %d", t);
+  if (r.n_tokens == 0) return DA_OK;
+  DA_REQUIRE(r.k && r.v && r.positions && (!r.n_q_heads || (r.q && r.q_out)), "da_paged_append: null pointer");
+  DA_REQUIRE(r.n_pages == 0 || (r.k_pages && r.v_pages), "da_paged_append: null pointer");
+  DA_REQUIRE((int64_t)r.n_sequences * r.pages_per_sequence == 0 || r.page_table, "da_paged_append: null pointer");
+  DA_REQUIRE(r.sequences || r.n_tokens <= r.n_sequences, "da_paged_append: %lld tokens for %d sequences",
+             (long long)r.n_tokens, r.n_sequences);
+  DA_REQUIRE(r.page_dtype == DA_E4M3 || (!r.k_scale && !r.v_scale), "da_paged_append: scales are for 8-bit pages");
+  const int64_t room = (int64_t)r.pages_per_sequence * r.page_size;
+  if (room > (int64_t)1 << 30) return fail(DA_ENOTSUP, "da_paged_append: sequences of up to 2^30 tokens");
+  const int e = elem_size(r.dtype), c = r.page_dtype == DA_E4M3 ? 1 : e, vec = 16 / e;
+  TurnArgs a = {};
+  const void *x[3] = {r.q, r.k, r.v};
+  void *y[3] = {r.q_out, r.k_pages, r.v_pages};
+  const int64_t *xs[3] = {r.q_strides, r.k_strides, r.v_strides};
+  bool vectors = whole_vectors(r.head_dim, r.rotary_dim, r.layout, vec);
+  for (int i = 0; i < 3; ++i) {
+    a.x[i] = (const char *)x[i];
+    a.y[i] = (char *)y[i];
+    a.x_tok_b[i] = xs[i][0] * e, a.x_head_b[i] = xs[i][1] * e;
+    if (i == 0) {
+      a.y_tok_b[0] = r.q_out_strides[0] * e, a.y_head_b[0] = r.q_out_strides[1] * e;
+      if (!r.n_q_heads) continue;
+      vectors = vectors && multiple((uintptr_t)y[0], 16) && multiple(r.q_out_strides[0], vec) &&
+                multiple(r.q_out_strides[1], vec);
+    } else {
+      a.y_batch_b[i] = r.page_strides[0] * c, a.y_tok_b[i] = r.page_strides[1] * c, a.y_head_b[i] = r.page_strides[2] * c;
+      vectors = vectors && multiple((uintptr_t)y[i], vec * c);
+      for (int j = 0; j < 3; ++j) vectors = vectors && multiple(r.page_strides[j], vec);
+    }
+    vectors = vectors && multiple((uintptr_t)x[i], 16) && multiple(xs[i][0], vec) && multiple(xs[i][1], vec);
+  }
+  a.row_end[0] = r.n_q_heads, a.row_end[1] = r.n_q_heads + r.n_kv_heads, a.row_end[2] = r.n_q_heads + 2 * r.n_kv_heads;
+  a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
+  a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type, a.pos_tok_stride = 1;
+  a.factor = r.factor, a.sign = 1.f;
+  a.table = r.page_table, a.table_stride = r.table_stride, a.table64 = r.table_type;
+  a.sequences = r.sequences, a.sequences64 = r.sequence_type;
+  a.n_sequences = r.n_sequences, a.n_pages = r.n_pages, a.max_tokens = (int32_t)room;
+  a.by_page = divisor_of(r.page_size);
+  a.scale[1] = r.k_scale, a.scale[2] = r.v_scale;
+  if (int rc = shape_rows(a, 1, r.n_tokens, vec, vectors, "da_paged_append")) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  if (r.page_dtype == DA_E4M3) {
+    if (r.dtype == DA_BF16) return launch_rows<BF16, E4M3, true>(a, vectors, s, "da_paged_append");
+    return launch_rows<F16, E4M3, true>(a, vectors, s, "da_paged_append");
+  }
+  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, true>(a, vectors, s, "da_paged_append");
+  if (r.dtype == DA_F16) return launch_rows<F16, F16, true>(a, vectors, s, "da_paged_append");
+  return launch_rows<F32, F32, true>(a, vectors, s, "da_paged_append");
+}

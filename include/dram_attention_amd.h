@@ -37,6 +37,7 @@ extern "C" {
 #define DA_F32 0
 #define DA_F16 1
 #define DA_BF16 2
+#define DA_E4M3 3 /* OCP e4m3, in the pages of da_paged_append and da_paged_attention only */
 /* integer types of index / mapping tensors, and of page_access_time */
 #define DA_I32 0
 #define DA_I64 1
@@ -613,6 +614,90 @@ int da_linear_block_tail(const void *attn, int attn_dim, const void *wo, const v
 /* out[0] = index of the largest of n fp32 values (16-byte aligned): the lowest of equal ones, a NaN
  * above everything (greedy decoding, examples/long-qa-chat/chat.py:255-262 of the reference). */
 int da_argmax(const float *x, int64_t n, int64_t *out, void *stream);
+
+/*
+ * Batches of sequences in HBM: queries and keys turned by their positions, keys and values stored in pages, and
+ * attention of one new token of every sequence over its pages.  (The reference keeps one sequence; its rotation is
+ * evaluation/dram-attention/model.py:126-136, its dense decode attention dram_attention/dram_attention.py:144-238.)
+ *
+ * Arguments come as a block, copied by the call; `args_bytes` is its size.  Strides are in elements.
+ */
+#define DA_ROTARY_INTERLEAVED 0 /* channels 2i and 2i + 1 turn together */
+#define DA_ROTARY_HALF 1        /* channels i and i + rotary_dim / 2 do */
+
+/*
+ * q (batch, tokens, n_q_heads, head_dim) and k (likewise, n_k_heads; either may have no heads) with the first
+ * rotary_dim channels of every head turned by position * freqs[i], cosine and sine times `factor`; angles in 64
+ * bits, the product in 32.  `inverse` turns the other way, which is the gradient.  Outputs may be the inputs
+ * themselves; otherwise they do not overlap them.  Any strides; 16-byte aligned rows are read and written by vectors.
+ */
+typedef struct da_rotate_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const double *freqs;      /* (rotary_dim / 2) radians per position */
+  const void *positions;    /* (batch, tokens) by position_strides, of position_type */
+  int64_t q_strides[3], k_strides[3], q_out_strides[3], k_out_strides[3]; /* batch, token, head */
+  int64_t position_strides[2];
+  int64_t batch, tokens;
+  int32_t n_q_heads, n_k_heads, head_dim, rotary_dim, layout, inverse, dtype, position_type;
+  float factor;
+  int32_t reserved;
+} da_rotate_args;
+int da_rotate(const void *args, size_t args_bytes, void *stream);
+
+/*
+ * Token t's key, turned as by da_rotate, and value go to page page_table[sequences[t], p / page_size], slot
+ * p % page_size, p = positions[t]; its query, if there are any, is turned into q_out.  A token whose p is negative or
+ * beyond its table row, whose sequence is none of the table's or whose page number is none of the pool's is not
+ * stored (its query is turned all the same).  No two tokens of a call share a sequence and a position.
+ *   k_pages, v_pages : (n_pages, page_size, n_kv_heads, head_dim), the same strides, of page_dtype: dtype, or DA_E4M3
+ *                      for 16-bit rows, which are divided by their kv head's scale (NULL: 1), clamped to 448 and rounded
+ *   page_table       : (n_sequences, pages_per_sequence), rows table_stride apart
+ *   sequences        : (n_tokens), or NULL: token t is of sequence t
+ */
+typedef struct da_paged_append_args {
+  const void *q, *k, *v;
+  void *q_out, *k_pages, *v_pages;
+  const double *freqs;
+  const void *page_table, *positions, *sequences;
+  const float *k_scale, *v_scale; /* (n_kv_heads) */
+  int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2]; /* token, head */
+  int64_t page_strides[3];                                            /* page, token, head */
+  int64_t table_stride, n_tokens;
+  int32_t n_pages, page_size, n_sequences, pages_per_sequence;
+  int32_t n_q_heads, n_kv_heads, head_dim, rotary_dim, layout, dtype, page_dtype;
+  int32_t table_type, position_type, sequence_type;
+  float factor;
+  int32_t reserved;
+} da_paged_append_args;
+int da_paged_append(const void *args, size_t args_bytes, void *stream);
+
+/*
+ * out[b, j] = softmax_t(q[b, j] . k_t * scale) v_t over the first lengths[b] tokens t of sequence b, whose keys and
+ * values lie in the pages of da_paged_append; query head j reads kv head j / (n_q_heads / n_kv_heads).  8-bit keys and
+ * values stand for themselves times their kv head's scale.  Lengths are clamped to 0 .. pages_per_sequence * page_size;
+ * tokens on pages that are none of the pool's do not count; a query for which no token counts gets zeros (lse -inf).
+ *   q         : (n_sequences, n_q_heads, head_dim), 16-byte aligned rows;  out: the same shape, contiguous, 16-byte aligned
+ *   lse       : optional (n_sequences, n_q_heads) fp32, natural log of the softmax denominator
+ *   workspace : da_paged_attention_workspace_bytes(args, args_bytes) bytes, 16-byte aligned, contents may be anything;
+ *               not shared by calls that may run at the same time
+ * head_dim 64, 96, 128 or 256 (DA_ENOTSUP otherwise).  The sums' order depends on shapes and lengths alone.
+ */
+typedef struct da_paged_attention_args {
+  const void *q, *k_pages, *v_pages, *page_table, *lengths;
+  const float *k_scale, *v_scale;
+  void *out;
+  float *lse;
+  void *workspace;
+  int64_t q_strides[2];    /* sequence, head */
+  int64_t page_strides[3]; /* page, token, head */
+  int64_t table_stride, workspace_bytes;
+  int32_t n_pages, page_size, n_sequences, pages_per_sequence;
+  int32_t n_q_heads, n_kv_heads, head_dim, dtype, page_dtype, table_type, length_type;
+  float scale;
+} da_paged_attention_args;
+size_t da_paged_attention_workspace_bytes(const void *args, size_t args_bytes);
+int da_paged_attention(const void *args, size_t args_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,221 @@
+"""Rotary positions on the GPU against their definition in 64 bits (tests/paged.py), forward and backward."""
+
+import pytest
+import torch
+
+from dram_attention_amd import rotary_frequencies, rotate, rotate_
+
+from . import paged as P
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype):
+    return torch.randn(*shape, generator=g).to(dtype).to(DEV)
+
+
+def check(got, x, positions, freqs, layout, factor=1.0):
+    want = P.turned(x, positions, freqs, layout, factor)
+    far = P.outside(got, want, P.turned_bound(x, x.dtype, factor, 2 * freqs.numel(), layout))
+    assert not far, far
+
+
+# (tokens, heads, kv heads, head_dim, rotary_dim)
+SHAPES = [(1, 32, 8, 128, 128), (1, 1, 1, 8, 2), (257, 5, 3, 80, 20), (64, 7, 1, 64, 64), (33, 4, 2, 128, 32),
+          (19, 3, 3, 96, 96), (10, 2, 1, 256, 256), (5, 3, 1, 512, 512), (9, 2, 2, 66, 66), (7, 40, 2, 24, 8),
+          (3, 2, 1, 5, 4), (300, 70, 10, 16, 16)]
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_rotate_against_the_definition(shape, dtype, layout):
+    T, Hq, H, D, R = shape
+    g = gen(T + D)
+    q, k = randn(g, T, Hq, D, dtype=dtype), randn(g, T, H, D, dtype=dtype)
+    freqs, _ = rotary_frequencies(R, 10000.0, device=DEV)
+    positions = torch.randint(-5, 200000, (T,), generator=g).to(torch.int32).to(DEV)
+    yq, yk = rotate(q, k, positions, freqs, layout=layout, factor=1.25)
+    check(yq, q, positions, freqs, layout, 1.25)
+    check(yk, k, positions, freqs, layout, 1.25)
+    assert torch.equal(yq[..., R:], q[..., R:]) and torch.equal(yk[..., R:], k[..., R:])
+    alone, none = rotate(q, None, positions.long(), freqs, layout=layout, factor=1.25)
+    assert none is None and torch.equal(alone, yq)
+    a, b = q.clone(), k.clone()
+    assert rotate_(a, b, positions, freqs, layout=layout, factor=1.25) == (a, b)
+    assert torch.equal(a, yq) and torch.equal(b, yk)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_far_positions_keep_their_angles(layout):
+    """2^27 positions: an angle is off by what two roundings in 64 bits are, 2^-52 * 2^27 rad, below fp32's."""
+    positions = torch.tensor([0, 1, 131071, 999_983, 16_777_217, 2 ** 27 - 1, -(2 ** 27 - 1)], dtype=torch.int64, device=DEV)
+    freqs, _ = rotary_frequencies(64, 500000.0, device=DEV)
+    x = randn(gen(0), 7, 2, 64, dtype=torch.float32)
+    check(rotate(x, None, positions, freqs, layout=layout)[0], x, positions, freqs, layout)
+
+
+def test_no_channel_turns():
+    x = randn(gen(1), 4, 2, 64, dtype=torch.bfloat16)
+    none = torch.empty(0, dtype=torch.float64, device=DEV)
+    assert torch.equal(rotate(x, None, torch.arange(4, device=DEV), none)[0], x)
+
+
+def test_empty_operands():
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    for shape in ((0, 4, 64), (3, 0, 64), (2, 0, 4, 64), (0, 5, 4, 64)):
+        x = torch.empty(shape, dtype=torch.bfloat16, device=DEV)
+        positions = torch.zeros(shape[:-2], dtype=torch.int32, device=DEV)
+        assert rotate(x, x, positions, freqs)[1].shape == x.shape
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_views_of_any_strides(dtype, layout):
+    g = gen(2)
+    B, S, H, D = 3, 21, 4, 64
+    freqs, _ = rotary_frequencies(D, device=DEV)
+    positions = torch.randint(0, 5000, (B, S), generator=g).to(torch.int32).to(DEV)
+    fused = randn(g, B, S, 3 * H + 1, D, dtype=dtype)
+    odd = randn(g, B * S * H * D + 1, dtype=dtype)[1:].view(B, S, H, D)                 # unaligned rows
+    for q, k in ((fused[:, :, :H], fused[:, :, H: 2 * H + 1]), (odd, odd[:, :, :1]),
+                 (randn(g, B, H, S, D, dtype=dtype).transpose(1, 2), fused[:, :, 1:2]),
+                 (randn(g, 1, S, H, D, dtype=dtype).expand(B, S, H, D), randn(g, B, S, 1, D, dtype=dtype).expand(B, S, H, D)),
+                 (randn(g, B, S, D, H, dtype=dtype).transpose(2, 3), randn(g, B, S, H, 2 * D, dtype=dtype)[..., ::2])):
+        yq, yk = rotate(q, k, positions, freqs, layout=layout)
+        check(yq, q, positions, freqs, layout)
+        check(yk, k, positions, freqs, layout)
+        wide = positions.t().contiguous().t().long()
+        assert torch.equal(rotate(q, k, wide, freqs, layout=layout)[0], yq)
+    both = fused.clone()
+    rotate_(both[:, :, :H], both[:, :, H: 2 * H], positions, freqs, layout=layout)
+    check(both[:, :, : 2 * H], fused[:, :, : 2 * H], positions, freqs, layout)
+    assert torch.equal(both[:, :, 2 * H:], fused[:, :, 2 * H:])
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients(dtype, layout):
+    g = gen(3)
+    B, S, Hq, H, D, R = 2, 13, 6, 2, 64, 48
+    freqs, factor = rotary_frequencies(R, scaling={"type": "yarn", "factor": 8.0, "original_length": 64}, device=DEV)
+    positions = torch.arange(100, 100 + S, device=DEV)
+    q, k = randn(g, B, S, Hq, D, dtype=dtype).requires_grad_(), randn(g, B, S, H, D, dtype=dtype).requires_grad_()
+    gq, gk = randn(g, B, S, Hq, D, dtype=dtype), randn(g, B, H, S, D, dtype=dtype).transpose(1, 2)
+    both = positions.expand(B, S)
+    yq, yk = rotate(q, k, positions, freqs, layout=layout, factor=factor)
+    dq, dk = torch.autograd.grad((yq, yk), (q, k), (gq, gk))
+    for got, gr in ((dq, gq), (dk, gk)):     # the transpose of the turn is the turn back
+        check(got, gr, -both, freqs, layout, factor)
+    # against differences of the (linear) function itself, summed in 64 bits
+    for y, x, gr, dx in ((yq, q, gq, dq), (yk, k, gk, dk)):
+        want = (y.detach().double() * gr.double()).sum()
+        got = (dx.double() * x.detach().double()).sum()
+        size = (y.detach().double() * gr.double()).abs().sum() + (dx.double() * x.detach().double()).abs().sum()
+        assert abs(got - want) <= 2 * P.HALF_STEP[dtype] * size
+    # one output used, one input that wants a gradient, and neither tensor's graph holding the other
+    dq1, = torch.autograd.grad(rotate(q, k, positions, freqs, layout=layout, factor=factor)[0], (q,), gq)
+    assert torch.equal(dq1, dq)
+    dk1, = torch.autograd.grad(rotate(q.detach(), k, positions, freqs, layout=layout, factor=factor)[1], (k,), gk)
+    assert torch.equal(dk1, dk)
+    dq2, = torch.autograd.grad(rotate(q, None, positions, freqs, layout=layout, factor=factor)[0], (q,), gq)
+    assert torch.equal(dq2, dq)
+
+
+def test_gradients_of_broadcast_rows_and_gradients_add_up():
+    g = gen(4)
+    S, H, D = 9, 6, 64
+    freqs, _ = rotary_frequencies(D, device=DEV)
+    positions = torch.arange(S, device=DEV)
+    one = randn(g, S, 1, D, dtype=torch.float32).requires_grad_()
+    y, _ = rotate(one.expand(S, H, D), None, positions, freqs)
+    gr = randn(g, S, 1, D, dtype=torch.float32)
+    got, = torch.autograd.grad(y, (one,), gr.expand(S, H, D))
+    want = P.turned(gr, -positions, freqs, "interleaved") * H
+    far = P.outside(got, want, (H + 1) * P.turned_bound(gr, torch.float32) + H * H * 2.0 ** -24 * want.abs())
+    assert not far, far
+
+
+def test_the_gradient_has_a_gradient():
+    g = gen(5)
+    q = randn(g, 5, 2, 64, dtype=torch.float32).requires_grad_()
+    gr = randn(g, 5, 2, 64, dtype=torch.float32).requires_grad_()
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(5, device=DEV)
+    y, _ = rotate(q, None, positions, freqs, layout="half")
+    dq, = torch.autograd.grad(y, (q,), gr, create_graph=True)
+    v = randn(g, 5, 2, 64, dtype=torch.float32)
+    back, = torch.autograd.grad(dq, (gr,), v)
+    check(back, v, positions, freqs, "half")
+
+
+def test_rotating_back_and_forth_through_a_graph_and_on_another_stream():
+    g = gen(6)
+    S, D = 50, 128
+    freqs, _ = rotary_frequencies(D, device=DEV)
+    q, k = randn(g, S, 8, D, dtype=torch.bfloat16), randn(g, S, 2, D, dtype=torch.bfloat16)
+    positions = torch.arange(S, device=DEV, dtype=torch.int32)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        rotate(q, k, positions, freqs)
+        ql, kl = q.clone().requires_grad_(), k.clone().requires_grad_()
+        gq, gk = torch.ones_like(q), torch.ones_like(k)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        yq, yk = rotate(ql, kl, positions, freqs)
+        dq, dk = torch.autograd.grad((yq, yk), (ql, kl), (gq, gk))
+    for step in range(3):
+        with torch.no_grad():
+            ql.copy_(randn(g, S, 8, D, dtype=torch.bfloat16))
+            gq.copy_(randn(g, S, 8, D, dtype=torch.bfloat16))
+            positions.add_(1000)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(yq, ql, positions, freqs, "interleaved")
+        check(yk, kl, positions, freqs, "interleaved")
+        check(dq, gq, -positions, freqs, "interleaved")
+        with torch.no_grad():
+            assert torch.equal(rotate(ql, kl, positions, freqs)[0], yq)
+
+
+def test_many_waves():
+    """More waves than a grid's first dimension has threads in one workgroup, heads in several windows."""
+    T, H, D = 20011, 9, 64
+    g = gen(7)
+    q = randn(g, T, H, D, dtype=torch.bfloat16)
+    freqs, _ = rotary_frequencies(32, device=DEV)
+    positions = torch.arange(T, device=DEV)
+    check(rotate(q, None, positions, freqs, layout="half")[0], q, positions, freqs, "half")
+
+
+def test_infinite_and_missing_values_stay_in_their_pairs():
+    x = torch.ones(1, 2, 64, dtype=torch.float32, device=DEV)
+    x[0, 0, 4] = float("nan")
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    y = rotate(x, None, torch.tensor([3], device=DEV), freqs)[0].cpu()
+    assert y[0, 0, 4:6].isnan().all() and y[0, 0].isnan().sum() == 2 and not y[0, 1].isnan().any()
+
+
+def test_refusals_that_need_a_gpu():
+    x = torch.zeros(4, 2, 64, device=DEV)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(4, device=DEV)
+    with pytest.raises(RuntimeError, match="freqs is on cpu"):
+        rotate(x, None, positions, freqs.cpu())
+    with pytest.raises(ValueError, match="share memory"):
+        rotate_(x[:, :1].expand(4, 2, 64), None, positions, freqs)
+    with pytest.raises(ValueError, match="share memory"):
+        rotate_(x, x, positions, freqs)
+    with pytest.raises(ValueError, match="dense rows"):
+        rotate_(torch.zeros(4, 2, 128, device=DEV)[..., ::2], None, positions, freqs)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        rotate_(x.clone().requires_grad_(), None, positions, freqs)

@@ -1,0 +1,256 @@
+"""Batches of sequences in HBM without a GPU: frequencies, refusals, the kernels' host side and its arithmetic."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from dram_attention_amd import (append_kv_pages_, kv_pages, paged_decode_attention, rotary_frequencies, rotate,
+                                rotate_)
+from dram_attention_amd.llama import rope_frequencies
+
+
+def freqs_of(n, *args, **more):
+    return rotary_frequencies(n, *args, device="cpu", **more)
+
+
+def test_frequencies_unscaled_and_llama3_are_the_models():
+    for scaled in (False, True):
+        freqs, factor = freqs_of(128, 500000.0, scaling={"type": "llama3"} if scaled else None)
+        assert factor == 1.0 and freqs.dtype == torch.float64 and freqs.shape == (64,)
+        # (the model's are formed in fp32: a power, a division and the blend)
+        assert torch.allclose(freqs.float(), rope_frequencies(128, 500000.0, scaled), rtol=1e-5, atol=0)
+
+
+def test_frequencies_by_their_formulas():
+    plain, _ = freqs_of(8, 10000.0)
+    assert torch.allclose(plain, torch.tensor([1.0, 0.1, 0.01, 0.001]).double(), rtol=1e-12)
+    assert torch.equal(freqs_of(8, 10000.0, {"type": "linear", "factor": 4.0})[0], plain / 4)
+    ntk, _ = freqs_of(8, 10000.0, {"type": "ntk", "factor": 16.0})
+    assert math.isclose(ntk[0], 1.0) and math.isclose(ntk[3], plain[3] / 16)        # slowest by the factor
+    yarn, factor = freqs_of(128, 10000.0, {"type": "yarn", "factor": 4.0, "original_length": 2048})
+    base, _ = freqs_of(128, 10000.0)
+    assert math.isclose(factor, 0.1 * math.log(4) + 1)
+    turns = 2048 * base / (2 * math.pi)
+    assert torch.allclose(yarn[turns > 40], base[turns > 40], rtol=1e-12)
+    assert torch.allclose(yarn[turns < 0.8], base[turns < 0.8] / 4, rtol=1e-12)
+    assert (yarn <= base).all() and (yarn >= base / 4 * (1 - 1e-12)).all() and (yarn[1:] < yarn[:-1]).all()
+    assert freqs_of(128, 10000.0, {"type": "yarn", "factor": 4.0, "original_length": 2048, "attention_factor": 1.5})[1] == 1.5
+    assert freqs_of(0)[0].numel() == 0
+
+
+@pytest.mark.parametrize("n, theta, scaling, match", [
+    (7, 1e4, None, "pairs"), (8, 1.0, None, "theta"), (8, 1e4, {"type": "linear"}, "factor"),
+    (8, 1e4, {"type": "linear", "factor": -1}, "factor"), (2, 1e4, {"type": "ntk", "factor": 2}, "two pairs"),
+    (8, 1e4, {"type": "yarn", "factor": 2}, "original_length"), (8, 1e4, {"type": "cubic"}, "unknown"),
+    (8, 1e4, {"type": "linear", "factor": 2, "beta": 1}, "beta"),
+    (8, 1e4, {"type": "llama3", "low_freq_factor": 4, "high_freq_factor": 1}, "high_freq_factor")])
+def test_frequencies_refuse(n, theta, scaling, match):
+    with pytest.raises(ValueError, match=match):
+        freqs_of(n, theta, scaling)
+
+
+def rotate_operands(**other):
+    a = dict(xq=torch.zeros(2, 3, 4, 64), xk=torch.zeros(2, 3, 1, 64), positions=torch.arange(3),
+             freqs=torch.zeros(32, dtype=torch.float64))
+    a.update(other)
+    return a
+
+
+@pytest.mark.parametrize("other, kind, match", [
+    ({}, RuntimeError, "GPU"),
+    ({"xq": torch.zeros(3, 64)}, ValueError, "xq must be"),
+    ({"xq": torch.zeros(2, 3, 4, 64, dtype=torch.float64)}, TypeError, "float32, float16 or bfloat16"),
+    ({"xk": torch.zeros(2, 3, 1, 64, dtype=torch.bfloat16)}, TypeError, "xk is"),
+    ({"xk": torch.zeros(2, 4, 1, 64)}, ValueError, "does not go with"),
+    ({"positions": torch.arange(4)}, ValueError, "positions"),
+    ({"positions": torch.zeros(3, 2, dtype=torch.int32)}, ValueError, "positions"),
+    ({"positions": torch.zeros(3)}, TypeError, "int32 or int64"),
+    ({"freqs": torch.zeros(32)}, TypeError, "float64"),
+    ({"freqs": torch.zeros(33, dtype=torch.float64)}, ValueError, "channels"),
+    ({"freqs": torch.zeros(64, dtype=torch.float64)[::2]}, ValueError, "contiguous"),
+    ({"freqs": None}, TypeError, "freqs"),
+    ({"layout": "both"}, ValueError, "layout"),
+])
+def test_rotate_refuses(other, kind, match):
+    with pytest.raises(kind, match=match):
+        rotate(**rotate_operands(**other))
+    with pytest.raises(kind, match=match):
+        rotate_(**rotate_operands(**other))
+
+
+def test_rotate_refuses_forward_mode():
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        rotate(**rotate_operands())
+
+
+def pages_on_cpu(dtype=torch.float32, **other):
+    k, v = kv_pages(6, 16, 2, 64, dtype=dtype, device="cpu")
+    a = dict(k_pages=k, v_pages=v, page_table=torch.zeros(3, 2, dtype=torch.int32))
+    a.update(other)
+    return a
+
+
+def test_pool_layout():
+    k, v = kv_pages(6, 16, 2, 64, device="cpu")
+    assert k.shape == v.shape == (6, 16, 2, 64) and k.dtype == torch.bfloat16 and k.stride() == v.stride()
+    assert k.stride() == (2 * 16 * 2 * 64, 128, 16 * 2 * 64, 1) and v.data_ptr() - k.data_ptr() == 128
+    for bad in (dict(dtype=torch.float64), dict(dtype=torch.int8)):
+        with pytest.raises(TypeError):
+            kv_pages(6, 16, 2, 64, device="cpu", **bad)
+    with pytest.raises(ValueError):
+        kv_pages(6, 0, 2, 64, device="cpu")
+
+
+X, I = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32)
+APPEND = [
+    ({}, RuntimeError, "GPU"),
+    ({"xk": torch.zeros(3, 2, 32)}, ValueError, "as the pages are"),
+    ({"xv": torch.zeros(3, 1, 64)}, ValueError, "as the pages are"),
+    ({"xv": X.bfloat16()}, TypeError, "xv is"),
+    ({"xk": X.half(), "xv": X.half()}, TypeError, "do not go with"),
+    ({"positions": I[:2]}, ValueError, "positions"),
+    ({"positions": X}, TypeError, "positions"),
+    ({"sequences": I[:2]}, ValueError, "sequences"),
+    ({"page_table": torch.zeros(4, 2, dtype=torch.int32)}, ValueError, "sequences="),
+    ({"page_table": torch.zeros(3, 2)}, TypeError, "page_table"),
+    ({"page_table": I}, ValueError, "page_table"),
+    ({"v_pages": torch.zeros(6, 16, 2, 64)}, ValueError, "same strides"),
+    ({"v_pages": torch.zeros(5, 16, 2, 64)}, ValueError, "must both be"),
+    ({"xq": torch.zeros(2, 4, 64)}, ValueError, "xq"),
+    ({"xq": torch.zeros(3, 4, 64, dtype=torch.half)}, TypeError, "xq is"),
+    ({"k_scale": torch.ones(2)}, ValueError, "8-bit"),
+    ({"freqs": torch.zeros(40, dtype=torch.float64)}, ValueError, "channels"),
+    ({"layout": None}, ValueError, "layout"),
+    ({"xk": X.clone().requires_grad_()}, RuntimeError, "no gradient"),
+]
+
+
+@pytest.mark.parametrize("other, kind, match", APPEND)
+def test_append_refuses(other, kind, match):
+    a = pages_on_cpu()
+    a.update(xk=X, xv=X, positions=I)
+    a.update(other)
+    with pytest.raises(kind, match=match):
+        append_kv_pages_(**a)
+
+
+def test_eight_bit_pages_refuse():
+    a = pages_on_cpu(torch.float8_e4m3fn)
+    with pytest.raises(TypeError, match="16-bit"):
+        append_kv_pages_(X, X, positions=I, **a)
+    with pytest.raises(TypeError, match="16-bit"):
+        paged_decode_attention(X, lengths=I, **a)
+    h = X.bfloat16()
+    for scale, kind in ((torch.ones(3), ValueError), (torch.ones(2).double(), TypeError), (torch.ones(4)[::2], ValueError)):
+        with pytest.raises(kind, match="k_scale"):
+            append_kv_pages_(h, h, positions=I, k_scale=scale, **a)
+        with pytest.raises(kind, match="v_scale"):
+            paged_decode_attention(h, lengths=I, v_scale=scale, **a)
+    with pytest.raises(RuntimeError, match="GPU"):
+        paged_decode_attention(h, lengths=I, k_scale=torch.ones(2), v_scale=torch.ones(2), **a)
+
+
+@pytest.mark.parametrize("other, kind, match", [
+    ({}, RuntimeError, "GPU"),
+    ({"xq": torch.zeros(3, 3, 64)}, ValueError, "multiple of 2 heads"),
+    ({"xq": torch.zeros(3, 0, 64)}, ValueError, "multiple of 2 heads"),
+    ({"xq": torch.zeros(2, 4, 64)}, ValueError, "3 sequences"),
+    ({"xq": torch.zeros(3, 1, 4, 64)}, ValueError, "xq"),
+    ({"xq": torch.zeros(3, 4, 64, dtype=torch.half)}, TypeError, "do not go with"),
+    ({"lengths": I[:2]}, ValueError, "lengths"),
+    ({"lengths": X}, TypeError, "lengths"),
+    ({"scale": math.inf}, ValueError, "finite"),
+    ({"scale": "1"}, TypeError, None),
+    ({"out": torch.zeros(3, 4, 32)}, ValueError, "out"),
+    ({"out": torch.zeros(3, 4, 64, dtype=torch.half)}, ValueError, "out"),
+    ({"lse": torch.zeros(3, 2)}, ValueError, "lse"),
+    ({"lse": torch.zeros(3, 4, dtype=torch.half)}, ValueError, "lse"),
+    ({"v_scale": torch.ones(2)}, ValueError, "8-bit"),
+    ({"xq": torch.zeros(3, 4, 64).requires_grad_()}, RuntimeError, "no gradient"),
+])
+def test_attention_refuses(other, kind, match):
+    a = pages_on_cpu()
+    a.update(xq=torch.zeros(3, 4, 64), lengths=I)
+    a.update(other)
+    with pytest.raises(kind, match=match):
+        paged_decode_attention(**a)
+
+
+class RotateArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "q_out", "k_out", "freqs", "positions")] + [
+        ("strides", ctypes.c_int64 * 14), ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("n_q_heads", "n_k_heads", "head_dim", "rotary_dim", "layout", "inverse", "dtype",
+                                      "position_type")] + [("factor", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class AppendArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out", "k_pages", "v_pages", "freqs", "page_table",
+                                               "positions", "sequences", "k_scale", "v_scale")] + [
+        ("strides", ctypes.c_int64 * 11), ("table_stride", ctypes.c_int64), ("n_tokens", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("n_pages", "page_size", "n_sequences", "pages_per_sequence", "n_q_heads",
+                                      "n_kv_heads", "head_dim", "rotary_dim", "layout", "dtype", "page_dtype",
+                                      "table_type", "position_type", "sequence_type")] + [
+        ("factor", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k_pages", "v_pages", "page_table", "lengths", "k_scale", "v_scale",
+                                               "out", "lse", "workspace")] + [
+        ("q_strides", ctypes.c_int64 * 2), ("page_strides", ctypes.c_int64 * 3), ("table_stride", ctypes.c_int64),
+        ("workspace_bytes", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("n_pages", "page_size", "n_sequences", "pages_per_sequence", "n_q_heads",
+                                      "n_kv_heads", "head_dim", "dtype", "page_dtype", "table_type", "length_type")] + [
+        ("scale", ctypes.c_float)]
+
+
+def call(lib, name, a):
+    return getattr(lib, name)(bytes(a), ctypes.sizeof(a), None)
+
+
+def test_c_entry_points_check_before_any_launch(lib):
+    for name in ("da_rotate", "da_paged_append", "da_paged_attention"):
+        assert getattr(lib, name)(None, 0, None) == -1
+        assert getattr(lib, name)(b"abc", 3, None) == -1 and b"argument block" in lib.da_last_error_string()
+    rot = dict(batch=1, tokens=4, n_q_heads=2, n_k_heads=1, head_dim=64, rotary_dim=64, dtype=2, factor=1.0)
+    for bad, code in (({}, -1), ({"dtype": 3}, -1), ({"rotary_dim": 63}, -1), ({"rotary_dim": 66}, -1), ({"layout": 2}, -1),
+                      ({"tokens": -1}, -1), ({"position_type": 5}, -1), ({"head_dim": 1024, "rotary_dim": 1024, "freqs": 16}, -2),
+                      ({"tokens": 1 << 40, "q": 16, "k": 16, "q_out": 16, "k_out": 16, "freqs": 16, "positions": 16}, -2),
+                      ({"tokens": 0, "freqs": 16}, 0)):
+        assert call(lib, "da_rotate", RotateArgs(**{**rot, **bad})) == code, bad
+    app = dict(n_pages=4, page_size=16, n_sequences=2, pages_per_sequence=3, n_kv_heads=2, head_dim=64, dtype=2,
+               page_dtype=2, n_tokens=2, k=16, v=16, k_pages=16, v_pages=16, page_table=16, positions=16)
+    for bad, code in (({"k": None}, -1), ({"n_tokens": 3}, -1), ({"page_dtype": 1}, -1), ({"dtype": 0, "page_dtype": 3}, -2),
+                      ({"page_size": 0}, -1), ({"n_q_heads": 2}, -1), ({"k_scale": 16}, -1), ({"sequence_type": 2}, -1),
+                      ({"page_size": 1 << 30}, -2), ({"rotary_dim": 64}, -1), ({"n_tokens": 0}, 0)):
+        assert call(lib, "da_paged_append", AppendArgs(**{**app, **bad})) == code, bad
+    att = dict(n_pages=4, page_size=16, n_sequences=2, pages_per_sequence=300, n_q_heads=4, n_kv_heads=2, head_dim=64,
+               dtype=2, page_dtype=2, q=16, k_pages=16, v_pages=16, page_table=16, lengths=16, out=16, scale=1.0)
+    for bad, code in (({"q": None}, -1), ({"head_dim": 80}, -2), ({"n_q_heads": 3}, -1), ({"page_dtype": 0}, -1),
+                      ({"dtype": 0, "page_dtype": 3}, -2), ({"v_scale": 16}, -1), ({"q": 8}, -1), ({}, -1),
+                      ({"workspace": 16, "workspace_bytes": 64}, -1), ({"page_size": 1 << 28}, -2), ({"length_type": 7}, -1),
+                      ({"q_strides": (ctypes.c_int64 * 2)(4, 64)}, -1), ({"n_sequences": 0}, 0)):
+        assert call(lib, "da_paged_attention", AttentionArgs(**{**att, **bad})) == code, bad
+    need = lib.da_paged_attention_workspace_bytes(bytes(AttentionArgs(**att)), ctypes.sizeof(AttentionArgs))
+    assert need > 0
+    assert lib.da_paged_attention_workspace_bytes(bytes(AttentionArgs(**{**att, "head_dim": 80})),
+                                                  ctypes.sizeof(AttentionArgs)) == 0
+    # (a batch that one workgroup a sequence finishes needs none)
+    assert lib.da_paged_attention_workspace_bytes(bytes(AttentionArgs(**{**att, "pages_per_sequence": 1})),
+                                                  ctypes.sizeof(AttentionArgs)) == 0
+
+
+def test_division_by_multiplication():
+    """The quotient that the kernels form for a token's page (csrc/paged_math.hpp), in its own integers."""
+    import random
+
+    rng = random.Random(0)
+    for d in [1, 2, 3, 5, 7, 16, 24, 100, 641, 65535, 65536, 65537, (1 << 30) - 1, 1 << 30] + [rng.randint(1, 1 << 30) for _ in range(300)]:
+        l = (d - 1).bit_length()
+        m = ((1 << l) - d << 32) // d + 1
+        assert m < 1 << 32
+        for n in [0, 1, d - 1, d, d + 1, (1 << 31) - 1, (1 << 31) - d if d < 1 << 31 else 0] + [rng.randrange(1 << 31) for _ in range(50)]:
+            assert ((m * n >> 32) + n) >> l == n // d, (n, d)
