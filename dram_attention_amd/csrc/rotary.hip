@@ -11,18 +11,19 @@
 // the millionth position of the fastest pair.  Whole turns go away in 64 bits, then quarters of a turn, and sine and
 // cosine of the rest are Taylor polynomials on |t| <= pi/4 (their next terms are below 2^-26).
 //
-// Bound: HBM; a row is read once and written once, 16 bytes a lane.  A wave takes one token and as many head rows
-// as make kPasses loads of 16 bytes a lane, all in flight while the lanes compute the token's angles, one pair
-// each, into LDS that only this wave reads: no barrier.  A token of many heads is several waves', which form its
-// angles again: they are 40 instructions a pair, and few tokens want many waves.
+// Bound: HBM; a row is read once and written once, 16 bytes a lane.  A workgroup takes a few tokens: its threads form
+// their angles, about one pair each, into LDS, while the first rows are on their way.  Its waves then take blocks of as
+// many head rows as 64 lanes hold, kInFlight blocks at a time; which token, tensor and rows a block is, is the same for
+// the whole wave and left to the scalar unit.
 #include "paged_math.hpp"
 
 namespace da {
 
 constexpr int kTurnThreads = 256;
 constexpr int kTurnWaves = kTurnThreads / 64;
-constexpr int kMaxPairs = 256;   // rotary_dim / 2
-constexpr int kPasses = 4;
+constexpr int kMaxPairs = 256;     // rotary_dim / 2
+constexpr int kMaxTurns = 1024;    // angles of a workgroup
+constexpr int kInFlight = 4;
 
 // Head rows: of q, then of k, then (append) of v.
 struct TurnArgs {
@@ -30,11 +31,12 @@ struct TurnArgs {
   char *y[3];
   int64_t x_batch_b[3], x_tok_b[3], x_head_b[3];
   int64_t y_batch_b[3], y_tok_b[3], y_head_b[3];   // (y of k and v in pages: page, token, head)
-  int32_t row_end[3];                              // head rows up to and with q's, k's, v's
+  int32_t rows[3];                                 // heads
+  int32_t block_end[3];                            // a token's blocks up to and with q's, k's, v's
   int32_t cols, lanes_shift;                       // items of a row; lanes that take them, as a power of two
   int32_t head_dim, rotary_dim, half;
-  int32_t windows, waves;                          // waves of a token, of all tokens
-  Divisor by_windows, by_tokens;                   // by_tokens: tokens of a batch
+  int32_t tokens, group;                           // of all batches; of a workgroup
+  Divisor by_tokens, by_blocks, by_pairs;          // tokens of a batch, blocks of a token, pairs of a row
   const double *freqs;
   const void *positions;
   int64_t pos_batch_stride, pos_tok_stride;
@@ -64,13 +66,19 @@ __device__ __forceinline__ void turn_of(double position, double freq, float fact
   s = factor * sign * (n & 2 ? -s1 : s1);
 }
 
+// A lane's kN elements as they are loaded: a 16-byte vector, or one element.
 template <typename T, int kN>
-__device__ __forceinline__ void load_row(const char *p, int at, float *f) {
-  if constexpr (kN == 1)
-    f[0] = load_elem<T>(p, at);
-  else
-    unpack<T>(load16(p + (int64_t)at * T::kBytes), f);
-}
+struct Held {
+  u32x4 v;
+  __device__ __forceinline__ void load(const char *p, int at) { v = load16(p + (int64_t)at * T::kBytes); }
+  __device__ __forceinline__ void values(float *f) const { unpack<T>(v, f); }
+};
+template <typename T>
+struct Held<T, 1> {
+  float v;
+  __device__ __forceinline__ void load(const char *p, int at) { v = load_elem<T>(p, at); }
+  __device__ __forceinline__ void values(float *f) const { f[0] = v; }
+};
 // kN values into elements of type TC; e4m3 ones divided by the head's scale first.
 template <typename TC, int kN>
 __device__ __forceinline__ void store_row(char *p, int at, float *f, float scale) {
@@ -96,22 +104,16 @@ __device__ __forceinline__ void store_row(char *p, int at, float *f, float scale
 // kN pairs, and behind those single ones that are copied.
 template <typename T, typename TC, int kN, bool kPairsInside, bool kPaged>
 __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArgs a) {
-  __shared__ float2 turns[kTurnWaves][kMaxPairs];
-  const int lane = threadIdx.x & 63;
-  const int wave = (int)(blockIdx.x * kTurnWaves + (threadIdx.x >> 6));
-  if (wave >= a.waves) return;
-  const int tok = divide(wave, a.by_windows), window = wave - tok * a.windows;
-  const int64_t batch = divide(tok, a.by_tokens), in_batch = tok - (int)batch * a.by_tokens.d;
-  const int64_t pos = load_index(a.positions, a.positions64, batch * a.pos_batch_stride + in_batch * a.pos_tok_stride);
+  __shared__ float2 turns[kMaxTurns];
+  __shared__ int64_t places[kTurnThreads];   // (append) byte offsets of the tokens in the pool, -1: not stored
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int first = (int)blockIdx.x * a.group, count = min(a.group, a.tokens - first);
   const int pairs = a.rotary_dim / 2;
-
-  const int lanes = 1 << a.lanes_shift, rows_per_pass = 64 >> a.lanes_shift;
-  const int first_row = window * rows_per_pass * kPasses + (lane >> a.lanes_shift);
-  const int rows = a.row_end[kPaged ? 2 : 1];
+  const int lanes = 1 << a.lanes_shift, rows_per_block = 64 >> a.lanes_shift;
+  const int row0 = lane >> a.lanes_shift, col0 = lane & (lanes - 1);
   const int turned_cols = kPairsInside ? a.rotary_dim / kN : pairs / kN;
-  const int col0 = lane & (lanes - 1);
+  const int blocks = a.by_blocks.d * count;
 
-  auto which = [&](int row) { return row < a.row_end[0] ? 0 : !kPaged || row < a.row_end[1] ? 1 : 2; };
   // An item's first element, and the second part's (pairs that lie apart).
   auto at_a = [&](int col) {
     if (kPairsInside) return col * kN;
@@ -120,101 +122,135 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
   };
   auto at_b = [&](int col) { return a.half ? pairs + col * kN : 2 * col + 1; };
 
-  // where the token's keys and values go
-  int64_t page_off = 0;
-  bool stored = true;
-  if constexpr (kPaged) {
-    const int64_t seq = a.sequences ? load_index(a.sequences, a.sequences64, tok) : tok;
-    stored = seq >= 0 && seq < a.n_sequences && pos >= 0 && pos < a.max_tokens;
-    const int at = stored ? (int)pos : 0;
-    const int page = divide(at, a.by_page);
-    const int64_t number = stored ? load_index(a.table, a.table64, seq * a.table_stride + page) : -1;
-    stored = number >= 0 && number < a.n_pages;
-    page_off = (stored ? number : 0) * a.y_batch_b[1] + (int64_t)(at - page * a.by_page.d) * a.y_tok_b[1];
-  }
-
-  // Rows wider than 64 items go in steps of 64.  (Lanes without an item stay: they have angles to form.)
-  for (int base = 0; base < a.cols; base += lanes) {
-    const int col = base + col0, end_row = col < a.cols ? rows : 0;
-    float fa[kPasses][kN], fb[kPasses][kN];
+  // What a block is (the same for the wave's lanes).
+  struct Block {
+    int tok, w, row;   // within the workgroup's tokens; tensor; first row
+    int64_t batch, in_batch;
+  };
+  auto block_at = [&](int j) {
+    Block x;
+    x.tok = divide(j, a.by_blocks);
+    const int within = j - x.tok * a.by_blocks.d;
+    x.w = within < a.block_end[0] ? 0 : !kPaged || within < a.block_end[1] ? 1 : 2;
+    x.row = (within - (x.w ? a.block_end[x.w - 1] : 0)) * rows_per_block;
+    x.batch = divide(first + x.tok, a.by_tokens);
+    x.in_batch = first + x.tok - (int)x.batch * a.by_tokens.d;
+    return x;
+  };
+  Held<T, kN> ha[kInFlight], hb[kInFlight];
+  auto load = [&](const Block &x, int col, int u) {
+    const int row = x.row + row0;
+    if (row >= a.rows[x.w] || col >= a.cols) return;
+    const char *p = a.x[x.w] + x.batch * a.x_batch_b[x.w] + x.in_batch * a.x_tok_b[x.w] + row * a.x_head_b[x.w];
+    ha[u].load(p, at_a(col));
+    if (!kPairsInside && col < turned_cols) hb[u].load(p, at_b(col));
+  };
+  auto store = [&](const Block &x, int col, int u) {
+    const int row = x.row + row0;
+    if (row >= a.rows[x.w] || col >= a.cols) return;
+    float fa[kN], fb[kN];
     const bool paired = !kPairsInside && col < turned_cols;
+    ha[u].values(fa);
+    if (paired) hb[u].values(fb);
+    if (col < turned_cols && x.w < 2) {
+      const float2 *turn = turns + x.tok * pairs + col * (kPairsInside ? kN / 2 : kN);
+      if constexpr (kPairsInside) {
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      const int row = first_row + u * rows_per_pass;
-      if (row >= end_row) continue;
-      const int w = which(row), head = row - (w ? a.row_end[w - 1] : 0);
-      const char *p = a.x[w] + batch * a.x_batch_b[w] + in_batch * a.x_tok_b[w] + head * a.x_head_b[w];
-      load_row<T, kN>(p, at_a(col), fa[u]);
-      if (paired) load_row<T, kN>(p, at_b(col), fb[u]);
-    }
-    if (base == 0) {
-      float2 *mine = turns[threadIdx.x >> 6];
-      for (int i = lane; i < pairs; i += 64) {
-        float c, s;
-        turn_of((double)pos, a.freqs[i], a.factor, a.sign, c, s);
-        mine[i] = make_float2(c, s);
+        for (int i = 0; i < kN; i += 2) rotate_pair(fa[i], fa[i + 1], turn[i / 2].x, turn[i / 2].y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) rotate_pair(fa[i], fb[i], turn[i].x, turn[i].y);
       }
-      __builtin_amdgcn_wave_barrier();
     }
-    const float2 *turn = turns[threadIdx.x >> 6];
-    float2 cs[kN];
-    if (col < turned_cols) {
-      constexpr int kPairs = kPairsInside ? kN / 2 : kN;
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) cs[i] = turn[col * kPairs + i];
+    if (!kPaged || x.w == 0) {
+      char *d = a.y[x.w] + x.batch * a.y_batch_b[x.w] + x.in_batch * a.y_tok_b[x.w] + row * a.y_head_b[x.w];
+      store_row<T, kN>(d, at_a(col), fa, 1.f);
+      if (paired) store_row<T, kN>(d, at_b(col), fb, 1.f);
+    } else {
+      const int64_t place = places[x.tok];
+      if (place < 0) return;
+      char *d = a.y[x.w] + place + row * a.y_head_b[x.w];
+      const float scale = TC::kBytes == 1 && a.scale[x.w] ? a.scale[x.w][row] : 1.f;
+      store_row<TC, kN>(d, at_a(col), fa, scale);
+      if (paired) store_row<TC, kN>(d, at_b(col), fb, scale);
     }
+  };
+
+  bool formed = false;
+  for (int base = 0; base < a.cols; base += lanes) {   // rows wider than 64 items go in steps of 64
+    const int col = base + col0;
+    // (a wave without a block still has angles to form and a barrier to reach)
+    for (int j0 = wave; j0 < blocks || !formed; j0 += kInFlight * kTurnWaves) {
 #pragma unroll
-    for (int u = 0; u < kPasses; ++u) {
-      const int row = first_row + u * rows_per_pass;
-      if (row >= end_row) continue;
-      const int w = which(row), head = row - (w ? a.row_end[w - 1] : 0);
-      if (col < turned_cols && w < 2) {
-        if constexpr (kPairsInside) {
-#pragma unroll
-          for (int i = 0; i < kN; i += 2) rotate_pair(fa[u][i], fa[u][i + 1], cs[i / 2].x, cs[i / 2].y);
-        } else {
-#pragma unroll
-          for (int i = 0; i < kN; ++i) rotate_pair(fa[u][i], fb[u][i], cs[i].x, cs[i].y);
+      for (int u = 0; u < kInFlight; ++u)
+        if (j0 + u * kTurnWaves < blocks) load(block_at(j0 + u * kTurnWaves), col, u);
+      if (!formed) {
+        formed = true;
+        auto position = [&](int tok) {
+          const int64_t batch = divide(first + tok, a.by_tokens);
+          return load_index(a.positions, a.positions64,
+                            batch * a.pos_batch_stride + (first + tok - (int)batch * a.by_tokens.d) * a.pos_tok_stride);
+        };
+        for (int i = threadIdx.x; i < count * pairs; i += kTurnThreads) {
+          const int tok = divide(i, a.by_pairs);
+          float c, s;
+          turn_of((double)position(tok), a.freqs[i - tok * pairs], a.factor, a.sign, c, s);
+          turns[i] = make_float2(c, s);
         }
+        if constexpr (kPaged) {
+          if (threadIdx.x < count) {
+            const int64_t pos = position(threadIdx.x);
+            const int64_t seq = a.sequences ? load_index(a.sequences, a.sequences64, first + threadIdx.x)
+                                            : (int64_t)(first + threadIdx.x);
+            int64_t place = -1;
+            if (seq >= 0 && seq < a.n_sequences && pos >= 0 && pos < a.max_tokens) {
+              const int page = divide((int)pos, a.by_page);
+              const int64_t number = load_index(a.table, a.table64, seq * a.table_stride + page);
+              if (number >= 0 && number < a.n_pages)
+                place = number * a.y_batch_b[1] + (int64_t)((int)pos - page * a.by_page.d) * a.y_tok_b[1];
+            }
+            places[threadIdx.x] = place;
+          }
+        }
+        __syncthreads();
       }
-      if (!kPaged || w == 0) {
-        char *d = a.y[w] + batch * a.y_batch_b[w] + in_batch * a.y_tok_b[w] + head * a.y_head_b[w];
-        store_row<T, kN>(d, at_a(col), fa[u], 1.f);
-        if (paired) store_row<T, kN>(d, at_b(col), fb[u], 1.f);
-      } else if (stored) {
-        char *d = a.y[w] + page_off + head * a.y_head_b[w];
-        const float scale = TC::kBytes == 1 && a.scale[w] ? a.scale[w][head] : 1.f;
-        store_row<TC, kN>(d, at_a(col), fa[u], scale);
-        if (paired) store_row<TC, kN>(d, at_b(col), fb[u], scale);
-      }
+#pragma unroll
+      for (int u = 0; u < kInFlight; ++u)
+        if (j0 + u * kTurnWaves < blocks) store(block_at(j0 + u * kTurnWaves), col, u);
     }
   }
 }
 
 static bool multiple(int64_t v, int of) { return v % of == 0; }
 
+// Workgroups that fill the chip; tokens are taken several at a time where there are more.
+constexpr int kTurnGrid = 2048;
+
 // Fills what follows from the shape; rows of whole 16-byte vectors (`vectors`) or element by element.
 static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool vectors, const char *what) {
-  const int n = vectors ? vec : 1;
+  const int n = vectors ? vec : 1, pairs = a.rotary_dim / 2;
   const bool inside = vectors && !a.half;
-  a.cols = inside ? a.head_dim / n : a.rotary_dim / 2 / n + (a.head_dim - a.rotary_dim) / n;
+  a.cols = inside ? a.head_dim / n : pairs / n + (a.head_dim - a.rotary_dim) / n;
   a.lanes_shift = 0;
   while (a.lanes_shift < 6 && (1 << a.lanes_shift) < a.cols) ++a.lanes_shift;
-  const int rows = a.row_end[2];
-  a.windows = (int)ceil_div(rows, (64 >> a.lanes_shift) * kPasses);
-  // (what is counted in 32 bits; with a few spare waves of the last workgroup)
-  const int64_t most = 0x7fffff00;
-  if (tokens > most / batch || batch * tokens > most / a.windows)
-    return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens, %d waves each, are too many", what, (long long)batch,
-                (long long)tokens, a.windows);
-  a.waves = (int32_t)(batch * tokens * a.windows);
-  a.by_windows = divisor_of(a.windows), a.by_tokens = divisor_of((int32_t)tokens);
+  int64_t blocks = 0;
+  for (int i = 0; i < 3; ++i) a.block_end[i] = (int32_t)(blocks += ceil_div(a.rows[i], 64 >> a.lanes_shift));
+  if (tokens > 0x7fffff00 / batch)   // (counted in 32 bits, a workgroup's tokens ahead)
+    return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens are too many", what, (long long)batch, (long long)tokens);
+  a.tokens = (int32_t)(batch * tokens);
+  // as many tokens as there are angles for every thread, while enough workgroups are left
+  a.group = 1;
+  while (a.group * 2 * (pairs > 1 ? pairs : 1) <= kTurnThreads && a.group * 2 <= 64 &&
+         a.tokens / (a.group * 2) >= kTurnGrid)
+    a.group *= 2;
+  a.by_tokens = divisor_of((int32_t)tokens), a.by_blocks = divisor_of((int32_t)blocks);
+  a.by_pairs = divisor_of(pairs > 1 ? pairs : 1);
   return DA_OK;
 }
 
 template <typename T, typename TC, bool kPaged>
 static int launch_rows(const TurnArgs &a, bool vectors, hipStream_t s, const char *what) {
-  const dim3 grid((unsigned)ceil_div(a.waves, kTurnWaves)), block(kTurnThreads);
+  const dim3 grid((unsigned)ceil_div(a.tokens, a.group)), block(kTurnThreads);
   if (!vectors)
     hipLaunchKernelGGL((rotary_rows_kernel<T, TC, 1, false, kPaged>), grid, block, 0, s, a);
   else if (a.half)
@@ -272,7 +308,7 @@ extern "C" int da_rotate(const void *args, size_t args_bytes, void *stream) {
     vectors = vectors && multiple((uintptr_t)x[i] | (uintptr_t)y[i], 16);
     for (int j = 0; j < 3; ++j) vectors = vectors && multiple(xs[i][j], vec) && multiple(ys[i][j], vec);
   }
-  a.row_end[0] = r.n_q_heads, a.row_end[1] = a.row_end[2] = r.n_q_heads + r.n_k_heads;
+  a.rows[0] = r.n_q_heads, a.rows[1] = r.n_k_heads;
   a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
   a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type;
   a.pos_batch_stride = r.position_strides[0], a.pos_tok_stride = r.position_strides[1];
@@ -331,7 +367,7 @@ extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream
     }
     vectors = vectors && multiple((uintptr_t)x[i], 16) && multiple(xs[i][0], vec) && multiple(xs[i][1], vec);
   }
-  a.row_end[0] = r.n_q_heads, a.row_end[1] = r.n_q_heads + r.n_kv_heads, a.row_end[2] = r.n_q_heads + 2 * r.n_kv_heads;
+  a.rows[0] = r.n_q_heads, a.rows[1] = a.rows[2] = r.n_kv_heads;
   a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
   a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type, a.pos_tok_stride = 1;
   a.factor = r.factor, a.sign = 1.f;
