@@ -23,7 +23,7 @@ constexpr int kTurnThreads = 256;
 constexpr int kTurnWaves = kTurnThreads / 64;
 constexpr int kMaxPairs = 256;     // rotary_dim / 2
 constexpr int kMaxTurns = 1024;    // angles of a workgroup
-constexpr int kInFlight = 4;
+constexpr int kInFlight = 3;
 
 // Head rows: of q, then of k, then (append) of v.
 struct TurnArgs {
@@ -67,20 +67,24 @@ __device__ __forceinline__ void turn_of(double position, double freq, float fact
 }
 
 // A lane's kN elements as they are loaded: a 16-byte vector, or one element.
-template <typename T, int kN>
+// kStream: rows come and go by streaming loads and stores.
+template <typename T, int kN, bool kStream>
 struct Held {
   u32x4 v;
-  __device__ __forceinline__ void load(const char *p, int at) { v = load16(p + (int64_t)at * T::kBytes); }
+  __device__ __forceinline__ void load(const char *p, int at) {
+    p += (int64_t)at * T::kBytes;
+    v = kStream ? load16_stream(p) : load16(p);
+  }
   __device__ __forceinline__ void values(float *f) const { unpack<T>(v, f); }
 };
-template <typename T>
-struct Held<T, 1> {
+template <typename T, bool kStream>
+struct Held<T, 1, kStream> {
   float v;
   __device__ __forceinline__ void load(const char *p, int at) { v = load_elem<T>(p, at); }
   __device__ __forceinline__ void values(float *f) const { f[0] = v; }
 };
 // kN values into elements of type TC; e4m3 ones divided by the head's scale first.
-template <typename TC, int kN>
+template <typename TC, int kN, bool kStream>
 __device__ __forceinline__ void store_row(char *p, int at, float *f, float scale) {
   if constexpr (TC::kBytes == 1) {
 #pragma unroll
@@ -95,14 +99,18 @@ __device__ __forceinline__ void store_row(char *p, int at, float *f, float scale
   } else if constexpr (kN == 1) {
     store_elem<TC>(p, at, f[0]);
   } else {
-    store16(p + (int64_t)at * TC::kBytes, pack_vec<TC>(f));
+    p += (int64_t)at * TC::kBytes;
+    if constexpr (kStream)
+      store16_stream(p, pack_vec<TC>(f));
+    else
+      store16(p, pack_vec<TC>(f));
   }
 }
 
 // kN: elements a load (a 16-byte vector, or 1 where a row's parts are no whole vectors).  kPairsInside: the
 // interleaved layout by vectors, whose pairs lie inside one; otherwise an item is the two vectors (or elements) of
 // kN pairs, and behind those single ones that are copied.
-template <typename T, typename TC, int kN, bool kPairsInside, bool kPaged>
+template <typename T, typename TC, int kN, bool kPairsInside, bool kPaged, bool kStream>
 __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArgs a) {
   __shared__ float2 turns[kMaxTurns];
   __shared__ int64_t places[kTurnThreads];   // (append) byte offsets of the tokens in the pool, -1: not stored
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
     x.in_batch = first + x.tok - (int)x.batch * a.by_tokens.d;
     return x;
   };
-  Held<T, kN> ha[kInFlight], hb[kInFlight];
+  Held<T, kN, kStream> ha[kInFlight], hb[kInFlight];
   auto load = [&](const Block &x, int col, int u) {
     const int row = x.row + row0;
     if (row >= a.rows[x.w] || col >= a.cols) return;
@@ -164,15 +172,15 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
     }
     if (!kPaged || x.w == 0) {
       char *d = a.y[x.w] + x.batch * a.y_batch_b[x.w] + x.in_batch * a.y_tok_b[x.w] + row * a.y_head_b[x.w];
-      store_row<T, kN>(d, at_a(col), fa, 1.f);
-      if (paired) store_row<T, kN>(d, at_b(col), fb, 1.f);
+      store_row<T, kN, kStream>(d, at_a(col), fa, 1.f);
+      if (paired) store_row<T, kN, kStream>(d, at_b(col), fb, 1.f);
     } else {
       const int64_t place = places[x.tok];
       if (place < 0) return;
       char *d = a.y[x.w] + place + row * a.y_head_b[x.w];
       const float scale = TC::kBytes == 1 && a.scale[x.w] ? a.scale[x.w][row] : 1.f;
-      store_row<TC, kN>(d, at_a(col), fa, scale);
-      if (paired) store_row<TC, kN>(d, at_b(col), fb, scale);
+      store_row<TC, kN, kStream>(d, at_a(col), fa, scale);
+      if (paired) store_row<TC, kN, kStream>(d, at_b(col), fb, scale);
     }
   };
 
@@ -224,7 +232,7 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
 static bool multiple(int64_t v, int of) { return v % of == 0; }
 
 // Workgroups that fill the chip; tokens are taken several at a time where there are more.
-constexpr int kTurnGrid = 2048;
+constexpr int kTurnGrid = 1024;
 
 // Fills what follows from the shape; rows of whole 16-byte vectors (`vectors`) or element by element.
 static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool vectors, const char *what) {
@@ -248,15 +256,24 @@ static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool 
   return DA_OK;
 }
 
+// Bytes read and written from which rows come and go by streaming: the last-level cache holds 256 MiB and would
+// keep none of them until they are used.  16384 tokens of 32/8 heads of 128 in bf16 (320 MiB) 72 -> 62 us, prompts of
+// 30720 tokens into pages (720 MiB) 163 -> 153; 4900 tokens of fp16 heads (58 MiB) 14 -> 20, their rows still in the cache.
+constexpr int64_t kStreamBytes = (int64_t)256 << 20;
+
 template <typename T, typename TC, bool kPaged>
 static int launch_rows(const TurnArgs &a, bool vectors, hipStream_t s, const char *what) {
   const dim3 grid((unsigned)ceil_div(a.tokens, a.group)), block(kTurnThreads);
-  if (!vectors)
-    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, 1, false, kPaged>), grid, block, 0, s, a);
-  else if (a.half)
-    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, T::kVec, false, kPaged>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((rotary_rows_kernel<T, TC, T::kVec, true, kPaged>), grid, block, 0, s, a);
+  const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
+  const bool stream = rows * a.tokens * a.head_dim * 2 * T::kBytes >= kStreamBytes;
+#define DA_TURN(n, inside, streaming) \
+  hipLaunchKernelGGL((rotary_rows_kernel<T, TC, n, inside, kPaged, streaming>), grid, block, 0, s, a)
+  if (!vectors) DA_TURN(1, false, false);
+  else if (a.half && stream) DA_TURN(T::kVec, false, true);
+  else if (a.half) DA_TURN(T::kVec, false, false);
+  else if (stream) DA_TURN(T::kVec, true, true);
+  else DA_TURN(T::kVec, true, false);
+#undef DA_TURN
   return launch_status(what);
 }
 
