@@ -32,6 +32,10 @@ namespace da {
 
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
+constexpr int kPagedMostShares = 1024;
+
+// Workgroups that a compute unit holds.
+constexpr int paged_resident(int row_bytes) { return row_bytes <= 128 ? 3 : 2; }
 
 struct PagedArgs {
   const char *q, *k, *v;
@@ -112,6 +116,16 @@ __device__ __forceinline__ void split_weights(float lo, float hi, uint32_t &firs
   }
 }
 
+__device__ __forceinline__ uint32_t load4_stream(const char *p) { return __builtin_nontemporal_load((const uint32_t *)p); }
+__device__ __forceinline__ u32x2 load8_stream(const char *p) { return __builtin_nontemporal_load((const u32x2 *)p); }
+
+// A barrier for what lies in LDS: loads from global memory stay in flight across it.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ __forceinline__ int sequence_length(const PagedArgs &a, int b) {
   const int64_t n = load_index(a.lengths, a.lengths64, b);
   return n < 0 ? 0 : n < a.max_tokens ? (int)n : a.max_tokens;
@@ -151,7 +165,7 @@ __device__ __forceinline__ void write_sums(const PagedArgs &a, bool whole, int64
 }
 
 template <typename T, typename KV, int kD>
-__global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPagedThreads, paged_resident(kD *KV::kBytes)) paged_attention_kernel(const PagedArgs a) {
   using Tile = PagedTile<T, KV, kD>;
   constexpr bool kWide = Tile::kWide;
   constexpr int kSets = Tile::kSets, kTokens = Tile::kTokens, kUnit = Tile::kUnit, kSteps = Tile::kSteps;
@@ -175,10 +189,18 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
   const float scale_log2 = a.scale_log2 * (KV::kBytes == 1 && a.k_scale ? a.k_scale[h] : 1.f);
   const float v_scale = KV::kBytes == 1 && a.v_scale ? a.v_scale[h] : 1.f;
 
+  auto write_nothing = [&](int i) {
+    for (int x = threadIdx.x; x < rows * kD; x += kPagedThreads) {
+      const int64_t row = (int64_t)i * a.n_q_heads + first_q + x / kD;
+      store_elem<T>(a.out, row * kD + x % kD, 0.f);
+      if (a.lse != nullptr && x % kD == 0) a.lse[row] = -INFINITY;
+    }
+  };
+
   // ---- this workgroup's share: units [u, u_end) of the line, from sequence b that has `before` units ahead of it
   int b = share, before = 0, u = 0, u_end = 0;
   if (a.shares == 0) {
-    u_end = (sequence_length(a, b) + kUnit - 1) / kUnit;
+    if (a.max_tokens > 0) u_end = (a.max_tokens - 1) / kUnit + 1;   // (its length is looked at below)
   } else {
     int total;
     if (a.n_seqs == 1) {
@@ -229,244 +251,279 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
     const int each = (total + a.shares - 1) / a.shares;
     u = min(share * each, total), u_end = min(u + each, total);
     // sequences without tokens, one after the other to the shares
-    for (int i = share; i < a.n_seqs; i += a.shares) {
-      if (sequence_length(a, i) > 0) continue;
-      for (int x = threadIdx.x; x < rows * kD; x += kPagedThreads) {
-        const int64_t row = (int64_t)i * a.n_q_heads + first_q + x / kD;
-        store_elem<T>(a.out, row * kD + x % kD, 0.f);
-        if (a.lse != nullptr && x % kD == 0) a.lse[row] = -INFINITY;
-      }
-    }
+    for (int i = share; i < a.n_seqs; i += a.shares)
+      if (sequence_length(a, i) == 0) write_nothing(i);
   }
-  if (a.shares == 0 && u_end == 0) {
-    for (int x = threadIdx.x; x < rows * kD; x += kPagedThreads) {
-      const int64_t row = (int64_t)b * a.n_q_heads + first_q + x / kD;
-      store_elem<T>(a.out, row * kD + x % kD, 0.f);
-      if (a.lse != nullptr && x % kD == 0) a.lse[row] = -INFINITY;
-    }
-  }
-
   const char *kbase = a.k + h * a.head_b, *vbase = a.v + h * a.head_b;
-  // (b stays in range even if a length changes while this runs)
-  for (; u < u_end && b < a.n_seqs; ++b) {
-    const int len = sequence_length(a, b), units = (len + kUnit - 1) / kUnit;
-    if (units == 0) continue;
-    const int from = u - before, to = min(u_end - before, units);
-    const int t0 = from * kUnit, t1 = min(to * kUnit, len);
-    const bool whole = from == 0 && to == units;
-    const int64_t table_row = b * a.table_stride;
 
-    u32x4 qv[kSteps];
-    {
-      const char *qp = a.q + b * a.q_seq_b + (first_q + (c < rows ? c : 0)) * a.q_head_b;
+  // A stretch of a sequence: its units [from, to) of `units`, tokens up to t1; `before` units lie ahead of the sequence
+  // on the line.  b = n_seqs: none.
+  struct Stretch {
+    int b, before, from, to, units, t1;
+  };
+  // The stretch at unit `u` of this share, in sequence b or one behind it.
+  auto stretch_at = [&](int b, int before, int u) {
+    Stretch x = {a.n_seqs, before, 0, 0, 0, 0};
+    if (u >= u_end) return x;
+    const int last = a.shares == 0 ? b + 1 : a.n_seqs;
+    for (; b < last; ++b) {   // (ends even if a length changes while this runs)
+      const int len = sequence_length(a, b);
+      x.units = (len + kUnit - 1) / kUnit;
+      if (x.units == 0) continue;
+      x.b = b, x.from = u - before, x.to = min(u_end - before, x.units);
+      x.t1 = min(x.to * kUnit, len);
+      break;
+    }
+    return x;
+  };
+  u32x4 qv[kSteps];
+  auto load_query = [&](int b) {
+    const char *qp = a.q + b * a.q_seq_b + (first_q + (c < rows ? c : 0)) * a.q_head_b;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        qv[s] = load16(qp + Tile::piece(s, g) * T::kBytes);
-        if (c >= rows) qv[s] = u32x4{0, 0, 0, 0};
+    for (int s = 0; s < kSteps; ++s) {
+      qv[s] = load16(qp + Tile::piece(s, g) * T::kBytes);
+      if (c >= rows) qv[s] = u32x4{0, 0, 0, 0};
+    }
+  };
+
+  float m, l;
+  f32x4 acc[kSlice];
+  uint32_t kk[kSets][kRowWords];
+  uint32_t vv[kHeld][kSliceWords];
+  uint32_t live = 0;   // of the tokens held: which count
+
+  // The number of the page of the lane's token of a tile in sequence b, -1 if it is none; whatever the sequence's length.
+  auto page_of = [&](int b, int tile) {
+    const int t = min(tile + (lane & (kTokens - 1)), a.max_tokens - 1);
+    const int64_t page = load_index(a.table, a.table64, b * a.table_stride + divide(t, a.by_page));
+    return page >= 0 && page < a.n_pages ? (int)page : -1;
+  };
+  // Byte offsets of the tile's tokens in the pool, -1 for those that do not count, for the wave's lanes to read.
+  auto publish = [&](int t1, int tile, int page) {
+    const int t = tile + (lane & (kTokens - 1)), slot = t - divide(t, a.by_page) * a.by_page.d;
+    if (lane < kTokens) offsets[wave][lane] = t < t1 && page >= 0 ? page * a.page_b + (int64_t)slot * a.tok_b : -1;
+    __builtin_amdgcn_wave_barrier();
+  };
+  auto load_keys = [&]() {
+#pragma unroll
+    for (int s = 0; s < kSets; ++s) {
+      const int64_t off = offsets[wave][16 * s + c];
+      const char *p = kbase + (off < 0 ? 0 : off);
+#pragma unroll
+      for (int w = 0; w + 4 <= kRowWords; w += 4) {
+        const u32x4 x = load16_stream(p + (w * 4 + g * 4) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kk[s][w + i] = x[i];
+      }
+      if constexpr (kRowWords % 4 == 2) {   // (96 e4m3)
+        const u32x2 x = load8_stream(p + (kRowWords - 2) * 16 + g * 8);
+        kk[s][kRowWords - 2] = x[0], kk[s][kRowWords - 1] = x[1];
       }
     }
-
-    float m = -INFINITY, l = 0.f;
-    f32x4 acc[kSlice];
+  };
+  auto load_values = [&]() {
+    live = 0;
 #pragma unroll
-    for (int j = 0; j < kSlice; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    uint32_t kk[kSets][kRowWords];
-    uint32_t vv[kHeld][kSliceWords];
-    uint32_t live = 0;   // of the tokens held: which count
-
-    // The page number of the lane's token of a tile (any valid table entry past the end).
-    auto page_of = [&](int tile) {
-      const int t = min(tile + (lane & (kTokens - 1)), t1 - 1);
-      return load_index(a.table, a.table64, table_row + divide(t, a.by_page));
-    };
-    // Byte offsets of the tile's tokens in the pool, -1 for those that do not count, for the wave's lanes to read.
-    auto publish = [&](int tile, int64_t page) {
-      const int t = tile + (lane & (kTokens - 1)), slot = t - divide(min(t, t1 - 1), a.by_page) * a.by_page.d;
-      const bool counts = t < t1 && page >= 0 && page < a.n_pages;
-      if (lane < kTokens) offsets[wave][lane] = counts ? page * a.page_b + (int64_t)slot * a.tok_b : -1;
-      __builtin_amdgcn_wave_barrier();
-    };
-    auto load_keys = [&]() {
-#pragma unroll
-      for (int s = 0; s < kSets; ++s) {
-        const int64_t off = offsets[wave][16 * s + c];
-        const char *p = kbase + (off < 0 ? 0 : off);
-#pragma unroll
-        for (int w = 0; w + 4 <= kRowWords; w += 4) {
-          const u32x4 x = load16(p + (w * 4 + g * 4) * 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) kk[s][w + i] = x[i];
-        }
-        if constexpr (kRowWords % 4 == 2) {   // (96 e4m3)
-          const u32x2 x = *(const u32x2 *)(p + (kRowWords - 2) * 16 + g * 8);
-          kk[s][kRowWords - 2] = x[0], kk[s][kRowWords - 1] = x[1];
-        }
-      }
-    };
-    auto load_values = [&]() {
-      live = 0;
-#pragma unroll
-      for (int x = 0; x < kHeld; ++x) {
-        const int64_t off = offsets[wave][16 * (x / 4) + 4 * g + x % 4];
-        live |= (off < 0 ? 0u : 1u) << x;
-        const char *p = vbase + (off < 0 ? 0 : off);
-        if constexpr (kD == 96) {
-          if constexpr (KV::kBytes == 1) {
-            vv[x][0] = *(const uint32_t *)(p + 4 * c);
-            vv[x][1] = *(const uint16_t *)(p + 64 + 2 * c);
-          } else if constexpr (KV::kBytes == 2) {
-            const u32x2 y = *(const u32x2 *)(p + 8 * c);
-            vv[x][0] = y[0], vv[x][1] = y[1];
-            vv[x][2] = *(const uint32_t *)(p + 128 + 4 * c);
-          } else {
-            const u32x4 y = load16(p + 16 * c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vv[x][i] = y[i];
-            const u32x2 z = *(const u32x2 *)(p + 256 + 8 * c);
-            vv[x][4] = z[0], vv[x][5] = z[1];
-          }
-        } else if constexpr (kSliceWords == 1) {
-          vv[x][0] = *(const uint32_t *)(p + 4 * c);
-        } else if constexpr (kSliceWords == 2) {
-          const u32x2 y = *(const u32x2 *)(p + 8 * c);
+    for (int x = 0; x < kHeld; ++x) {
+      const int64_t off = offsets[wave][16 * (x / 4) + 4 * g + x % 4];
+      live |= (off < 0 ? 0u : 1u) << x;
+      const char *p = vbase + (off < 0 ? 0 : off);
+      if constexpr (kD == 96) {
+        if constexpr (KV::kBytes == 1) {
+          vv[x][0] = load4_stream(p + 4 * c);
+          vv[x][1] = *(const uint16_t *)(p + 64 + 2 * c);
+        } else if constexpr (KV::kBytes == 2) {
+          const u32x2 y = load8_stream(p + 8 * c);
           vv[x][0] = y[0], vv[x][1] = y[1];
+          vv[x][2] = load4_stream(p + 128 + 4 * c);
         } else {
+          const u32x4 y = load16_stream(p + 16 * c);
 #pragma unroll
-          for (int w = 0; w < kSliceWords; w += 4) {
-            const u32x4 y = load16(p + (kSliceWords * c + w) * 4);
+          for (int i = 0; i < 4; ++i) vv[x][i] = y[i];
+          const u32x2 z = load8_stream(p + 256 + 8 * c);
+          vv[x][4] = z[0], vv[x][5] = z[1];
+        }
+      } else if constexpr (kSliceWords == 1) {
+        vv[x][0] = load4_stream(p + 4 * c);
+      } else if constexpr (kSliceWords == 2) {
+        const u32x2 y = load8_stream(p + 8 * c);
+        vv[x][0] = y[0], vv[x][1] = y[1];
+      } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vv[x][w + i] = y[i];
-          }
+        for (int w = 0; w < kSliceWords; w += 4) {
+          const u32x4 y = load16_stream(p + (kSliceWords * c + w) * 4);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vv[x][w + i] = y[i];
         }
       }
-    };
+    }
+  };
 
-    // S^T of the tile in kk
-    auto scores = [&](f32x4 *st) {
+  // S^T of the tile in kk
+  auto scores = [&](f32x4 *st) {
 #pragma unroll
-      for (int s = 0; s < kSets; ++s) {
-        f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
-        if constexpr (kWide) {
-#pragma unroll
-          for (int i = 0; i < 4 * kSteps; ++i) {   // two chains
-            f32x4 &z = i & 1 ? y : x;
-            z = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(kk[s][i]), as_f32(qv[i / 4][i % 4]), z, 0, 0, 0);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
-            u32x4 ka;
-            if constexpr (KV::kBytes == 1) {
-              const uint32_t w0 = kk[s][2 * i], w1 = kk[s][2 * i + 1];
-              ka = u32x4{widen_e4m3<T, false>(w0), widen_e4m3<T, true>(w0), widen_e4m3<T, false>(w1),
-                         widen_e4m3<T, true>(w1)};
-            } else {
-              ka = u32x4{kk[s][4 * i], kk[s][4 * i + 1], kk[s][4 * i + 2], kk[s][4 * i + 3]};
-            }
-            f32x4 &z = i & 1 ? y : x;
-            z = MatrixOps<T>::k32(ka, qv[i], z);
-          }
-        }
-        st[s] = x + y;
-      }
-    };
-
-    // Weights of the tile's scores; O^T += V^T P^T
-    auto weigh = [&](const f32x4 *st) {
-      float p[kHeld];
-      float top = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kHeld; ++x) {
-        p[x] = live >> x & 1 ? st[x / 4][x % 4] * scale_log2 : -INFINITY;
-        top = fmaxf(top, p[x]);
-      }
-      if (__any(top > m + (Range::kSlack + Range::kBias))) {   // rare
-        float mx = top - Range::kBias;
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
-        const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
-        m = mx;
-        l *= alpha;
-#pragma unroll
-        for (int j = 0; j < kSlice; ++j) acc[j] *= alpha;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int x = 0; x < kHeld; ++x) {
-        p[x] = fast_exp2(p[x] - ref);
-        l += p[x];
-      }
-      // values of tokens that do not count are memory nobody vouches for: 0 * NaN must not arise
-      if (__any(live != (1u << kHeld) - 1)) {
-#pragma unroll
-        for (int x = 0; x < kHeld; ++x)
-#pragma unroll
-          for (int w = 0; w < kSliceWords; ++w) vv[x][w] = live >> x & 1 ? vv[x][w] : 0u;
-      }
+    for (int s = 0; s < kSets; ++s) {
+      f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
       if constexpr (kWide) {
 #pragma unroll
-        for (int x = 0; x < kHeld; ++x)
-#pragma unroll
-          for (int j = 0; j < kSlice; ++j)
-            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[x], acc[j], 0, 0, 0);
-      } else {
-        u32x4 p1, p2;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t first, rest;
-          split_weights<T>(p[2 * i], p[2 * i + 1], first, rest);
-          p1[i] = first, p2[i] = rest;
+        for (int i = 0; i < 4 * kSteps; ++i) {   // two chains
+          f32x4 &z = i & 1 ? y : x;
+          z = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(kk[s][i]), as_f32(qv[i / 4][i % 4]), z, 0, 0, 0);
         }
+      } else {
 #pragma unroll
-        for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
-          uint32_t w[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            if constexpr (KV::kBytes == 1)
-              w[x] = jj & 1 ? widen_e4m3<T, true>(vv[x][jj / 2]) : widen_e4m3<T, false>(vv[x][jj / 2]);
-            else
-              w[x] = vv[x][jj];
+        for (int i = 0; i < kSteps; ++i) {
+          u32x4 ka;
+          if constexpr (KV::kBytes == 1) {
+            const uint32_t w0 = kk[s][2 * i], w1 = kk[s][2 * i + 1];
+            ka = u32x4{widen_e4m3<T, false>(w0), widen_e4m3<T, true>(w0), widen_e4m3<T, false>(w1),
+                       widen_e4m3<T, true>(w1)};
+          } else {
+            ka = u32x4{kk[s][4 * i], kk[s][4 * i + 1], kk[s][4 * i + 2], kk[s][4 * i + 3]};
           }
-          u32x4 even, odd;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-            odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
-          }
-          acc[2 * jj] = MatrixOps<T>::k32(even, p1, acc[2 * jj]);
-          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p1, acc[2 * jj + 1]);
-          acc[2 * jj] = MatrixOps<T>::k32(even, p2, acc[2 * jj]);
-          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p2, acc[2 * jj + 1]);
+          f32x4 &z = i & 1 ? y : x;
+          z = MatrixOps<T>::k32(ka, qv[i], z);
         }
       }
-    };
+      st[s] = x + y;
+    }
+  };
 
-    int tile = t0 + wave * kTokens;
-    if (tile < t1) {
-      int64_t page = page_of(tile), next = page_of(tile + kUnit);
-      publish(tile, page);
+  // Weights of the tile's scores; O^T += V^T P^T
+  auto weigh = [&](const f32x4 *st) {
+    float p[kHeld];
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) {
+      p[x] = live >> x & 1 ? st[x / 4][x % 4] * scale_log2 : -INFINITY;
+      top = fmaxf(top, p[x]);
+    }
+    if (__any(top > m + (Range::kSlack + Range::kBias))) {   // rare
+      float mx = top - Range::kBias;
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
+      const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
+      m = mx;
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < kSlice; ++j) acc[j] *= alpha;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int x = 0; x < kHeld; ++x) {
+      p[x] = fast_exp2(p[x] - ref);
+      l += p[x];
+    }
+    // values of tokens that do not count are memory nobody vouches for: 0 * NaN must not arise
+    if (__any(live != (1u << kHeld) - 1)) {
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x)
+#pragma unroll
+        for (int w = 0; w < kSliceWords; ++w) vv[x][w] = live >> x & 1 ? vv[x][w] : 0u;
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x)
+#pragma unroll
+        for (int j = 0; j < kSlice; ++j)
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[x], acc[j], 0, 0, 0);
+    } else {
+      u32x4 p1, p2;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t first, rest;
+        split_weights<T>(p[2 * i], p[2 * i + 1], first, rest);
+        p1[i] = first, p2[i] = rest;
+      }
+#pragma unroll
+      for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
+        uint32_t w[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          if constexpr (KV::kBytes == 1)
+            w[x] = jj & 1 ? widen_e4m3<T, true>(vv[x][jj / 2]) : widen_e4m3<T, false>(vv[x][jj / 2]);
+          else
+            w[x] = vv[x][jj];
+        }
+        u32x4 even, odd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+          odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+        }
+        acc[2 * jj] = MatrixOps<T>::k32(even, p1, acc[2 * jj]);
+        acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p1, acc[2 * jj + 1]);
+        acc[2 * jj] = MatrixOps<T>::k32(even, p2, acc[2 * jj]);
+        acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p2, acc[2 * jj + 1]);
+      }
+    }
+  };
+
+  // A wave's first tile of a stretch is loaded before the sums of the stretch ahead are put together.
+  auto first_tile = [&](const Stretch &x) { return x.from * kUnit + wave * kTokens; };
+  if (u >= u_end) {
+    if (a.shares == 0) write_nothing(b);   // (a table or a pool without pages)
+    return;
+  }
+  // (the first loads wait for no length)
+  load_query(b);
+  const int tile0 = (u - before) * kUnit + wave * kTokens, page0 = page_of(b, tile0);
+  int next = page_of(b, tile0 + kUnit);   // page numbers of the tile behind the one that is loaded
+  Stretch cur = stretch_at(b, before, u);
+  if (cur.b != b) {
+    if (a.shares == 0) write_nothing(b);
+    return;   // (of a share: only if a length has changed since)
+  }
+  publish(cur.t1, tile0, page0);
+  load_keys();
+  load_values();
+  for (;;) {
+    Stretch nxt = {a.n_seqs, 0, 0, 0, 0, 0};
+    if (a.shares != 0) nxt = stretch_at(cur.b + 1, cur.before + cur.units, cur.before + cur.to);
+    const bool more = nxt.b < a.n_seqs;
+    int page0 = -1, page1 = -1;
+    if (more) {
+      page0 = page_of(nxt.b, first_tile(nxt));
+      page1 = page_of(nxt.b, first_tile(nxt) + kUnit);
+    }
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < kSlice; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int tile = first_tile(cur);
+    const bool any = tile < cur.t1;
+    for (; tile + kUnit < cur.t1; tile += kUnit) {
+      f32x4 st[kSets];
+      const int page = page_of(cur.b, tile + 2 * kUnit);
+      scores(st);
+      publish(cur.t1, tile + kUnit, next);
       load_keys();
+      weigh(st);
       load_values();
-      for (; tile < t1; tile += kUnit) {
-        f32x4 st[kSets];
-        page = page_of(tile + 2 * kUnit);
-        scores(st);
-        publish(tile + kUnit, next);
+      next = page;
+    }
+    {
+      f32x4 st[kSets];
+      if (any) scores(st);
+      if (more) {
+        publish(nxt.t1, first_tile(nxt), page0);
         load_keys();
-        weigh(st);
+      }
+      if (any) weigh(st);
+      if (more) {
         load_values();
-        next = page;
+        load_query(nxt.b);
+        next = page1;
       }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
     // ---- the waves' sums together
-    const int64_t part = (((int64_t)hg * a.shares + share) * 2 + (from == 0 ? 1 : 0)) * 16;
+    const bool whole = cur.from == 0 && cur.to == cur.units;
+    const int64_t part = (((int64_t)hg * a.shares + share) * 2 + (cur.from == 0 ? 1 : 0)) * 16;
 #pragma unroll
     for (int j0 = 0; j0 < kSlice; j0 += kJ) {
-      __syncthreads();   // (what the last pass or sequence left there has been read)
+      lds_barrier();   // (what the last pass or stretch left there has been read)
       if (c < rows) {
         if (g == 0) sm_m[wave][c] = m, sm_l[wave][c] = l;
 #pragma unroll
@@ -474,7 +531,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
           for (int j = 0; j < kJ; ++j) sm_acc[wave][c][(4 * g + i) * kJ + j] = acc[j0 + j][i];
       }
-      __syncthreads();
+      lds_barrier();
       const int row = threadIdx.x >> 4, r = threadIdx.x & 15;
       if (row < rows) {
         float mx = sm_m[0][row];
@@ -490,12 +547,12 @@ __global__ void __launch_bounds__(kPagedThreads) paged_attention_kernel(const Pa
 #pragma unroll
           for (int j = 0; j < kJ; ++j) at[j] += sm_acc[w][row][r * kJ + j] * by;
         }
-        write_sums<T, Tile, kJ>(a, whole, (int64_t)b * a.n_q_heads + first_q + row, part + row, kD, r, j0, mx, sum,
+        write_sums<T, Tile, kJ>(a, whole, (int64_t)cur.b * a.n_q_heads + first_q + row, part + row, kD, r, j0, mx, sum,
                                 v_scale, at);
       }
     }
-    u = before + to;
-    before += units;
+    if (!more) break;
+    cur = nxt;
   }
 }
 
@@ -505,7 +562,7 @@ template <typename T, int kD>
 __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedArgs a, const bool by_border) {
   constexpr int kLanes = kD / 4, kParts = kPagedThreads / kLanes;
   __shared__ __align__(16) float sums[kParts][kD];
-  __shared__ float red[kPagedWaves], ls[kParts];
+  __shared__ float red[kPagedWaves], ls[kPagedWaves], weight[kPagedMostShares];
   const int hq = (int)(blockIdx.x % (unsigned)a.n_q_heads), at = (int)(blockIdx.x / (unsigned)a.n_q_heads);
   const int total = a.prefix[a.n_seqs];
   const int each = (total + a.shares - 1) / a.shares;
@@ -529,31 +586,40 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedAr
   const int64_t hg = (int64_t)h * a.groups + rr / 16;
   auto row = [&](int i) { return ((hg * a.shares + s0 + i) * 2 + (i == 0 ? 1 : 0)) * 16 + rr % 16; };
 
-  float mx = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kPagedThreads) mx = fmaxf(mx, a.part_ml[row(i) * 2]);
+  // the parts' maxima and sums: each thread a few, then by the block
+  constexpr int kOwn = kPagedMostShares / kPagedThreads;
+  float m[kOwn], mx = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int x = 0; x < kOwn; ++x) {
+    const int i = threadIdx.x + x * kPagedThreads;
+    m[x] = i < n ? a.part_ml[row(i) * 2] : -INFINITY;
+    mx = fmaxf(mx, m[x]);
+  }
   mx = group_max<64>(mx);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
   __syncthreads();
   mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int x = 0; x < kOwn; ++x) {
+    const int i = threadIdx.x + x * kPagedThreads;
+    if (i >= n) break;
+    const float by = mx == -INFINITY ? 1.f : fast_exp2(m[x] - mx);
+    weight[i] = by;
+    l += a.part_ml[row(i) * 2 + 1] * by;
+  }
+  l = group_sum<64>(l);
+  if ((threadIdx.x & 63) == 0) ls[threadIdx.x >> 6] = l;
+  __syncthreads();
+  l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
 
   const int part = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
-  float l = 0.f;
-  f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
   if (part < kParts) {
-    for (int i = part; i < n; i += kParts) {
-      const int64_t x = row(i);
-      const float m = a.part_ml[x * 2];
-      const float by = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
-      l += a.part_ml[x * 2 + 1] * by;
-      sum += *(const f32x4 *)(a.part_acc + x * kD + d) * by;
-    }
+    f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int i = part; i < n; i += kParts) sum += *(const f32x4 *)(a.part_acc + row(i) * kD + d) * weight[i];
     *(f32x4 *)&sums[part][d] = sum;
   }
-  if (part < kParts && d == 0) ls[part] = l;   // (the same in every lane of a part)
   __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) l += ls[i];
   const int64_t out_row = (int64_t)b * a.n_q_heads + hq;
   const float v_scale = a.v_scale ? a.v_scale[h] : 1.f;
   for (int x = threadIdx.x; x < kD; x += kPagedThreads) {
