@@ -23,11 +23,11 @@ static PagedPlan paged_plan(const da_paged_attention_args &r) {
   p.groups = (int32_t)ceil_div(rep, 16);
   const int64_t head_groups = (int64_t)r.n_kv_heads * p.groups;
   const int64_t room = paged_room(r), units = ceil_div(room, r.dtype == DA_F32 ? 64 : 128);
-  const int row_bytes = r.head_dim * (r.page_dtype == DA_E4M3 ? 1 : elem_size(r.dtype));
-  int64_t shares = kComputeUnits * paged_resident(row_bytes) / head_groups;
+  const int bytes = r.page_dtype == DA_E4M3 ? 1 : elem_size(r.dtype);
+  int64_t shares = kComputeUnits * paged_resident(r.head_dim, bytes) / head_groups;
   if (shares > units * r.n_sequences) shares = units * r.n_sequences;
   if (room <= kPagedDirect || shares <= 1) return p;
-  static_assert(kComputeUnits * paged_resident(1) <= kPagedMostShares, "the join's threads hold that many");
+  static_assert(kComputeUnits * paged_resident(64, 1) <= kPagedMostShares, "the join's threads hold that many");
   p.shares = (int32_t)shares;
   const int64_t rows = head_groups * shares * 2 * 16;
   p.prefix_bytes = (size_t)ceil_div(((int64_t)r.n_sequences + 1) * 4, 16) * 16;

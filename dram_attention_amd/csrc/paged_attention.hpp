@@ -35,7 +35,9 @@ constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kPagedMostShares = 1024;
 
 // Workgroups that a compute unit holds.
-constexpr int paged_resident(int row_bytes) { return row_bytes <= 128 ? 3 : 2; }
+constexpr int paged_resident(int head_dim, int bytes) {
+  return head_dim == 64 ? 4 : head_dim == 96 || (head_dim == 128 && bytes == 1) ? 3 : head_dim == 128 || bytes == 1 ? 2 : 1;
+}
 
 struct PagedArgs {
   const char *q, *k, *v;
@@ -165,7 +167,7 @@ __device__ __forceinline__ void write_sums(const PagedArgs &a, bool whole, int64
 }
 
 template <typename T, typename KV, int kD>
-__global__ void __launch_bounds__(kPagedThreads, paged_resident(kD *KV::kBytes)) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes)) paged_attention_kernel(const PagedArgs a) {
   using Tile = PagedTile<T, KV, kD>;
   constexpr bool kWide = Tile::kWide;
   constexpr int kSets = Tile::kSets, kTokens = Tile::kTokens, kUnit = Tile::kUnit, kSteps = Tile::kSteps;
