@@ -4,8 +4,12 @@
 namespace da {
 
 constexpr int kComputeUnits = 256;
-// Tokens up to which a sequence is one workgroup's: joining costs a launch of its own.
-constexpr int kPagedDirect = 512;
+// A sequence is one workgroup's where the table holds no more than this many tokens of it: joining costs a launch and
+// sharing out a scan.  Up to 512 tokens it always pays (one sequence of 256 of 32/8 heads 6.5 instead of 9.0 us, of 512 9.3 and
+// 9.1, 64 of 512 22.7 and 27.2), up to 1024 where there are workgroups for every compute unit twice (64 sequences of 1024
+// 42.7 and 47.0, of unlike lengths 33.9 and 36.1, but 16 of them 21.5 and 18.1); beyond, unlike lengths leave most of the chip
+// waiting for the longest (64 of up to 4096 124 and 85).
+constexpr int kPagedDirect = 512, kPagedDirectMany = 1024;
 
 constexpr int64_t kPagedMostTokens = (int64_t)1 << 30;   // of a sequence: tiles ahead are counted in 32 bits
 
@@ -26,7 +30,8 @@ static PagedPlan paged_plan(const da_paged_attention_args &r) {
   const int bytes = r.page_dtype == DA_E4M3 ? 1 : elem_size(r.dtype);
   int64_t shares = kComputeUnits * paged_resident(r.head_dim, bytes) / head_groups;
   if (shares > units * r.n_sequences) shares = units * r.n_sequences;
-  if (room <= kPagedDirect || shares <= 1) return p;
+  const bool many = r.n_sequences * head_groups >= 2 * kComputeUnits;
+  if (room <= (many ? kPagedDirectMany : kPagedDirect) || shares <= 1) return p;
   static_assert(kComputeUnits * paged_resident(64, 1) <= kPagedMostShares, "the join's threads hold that many");
   p.shares = (int32_t)shares;
   const int64_t rows = head_groups * shares * 2 * 16;
