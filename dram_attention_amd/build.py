@@ -175,7 +175,9 @@ def build_host_calls(library: Path) -> Path:
     out = library.with_name(HOST_PATH.name)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{sysconfig.get_paths()['include']}",
            "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
+           "-isystem", str(Path(_hipcc()).resolve().parents[1] / "include"), "-D__HIP_PLATFORM_AMD__",
            str(CSRC / "host_calls.cpp"), "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-lc10_hip",
            f"-L{library.parent}", "-ldramattn", "-Wl,-rpath,$ORIGIN"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:

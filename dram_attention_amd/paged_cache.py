@@ -47,8 +47,7 @@ def append_kv_pages_(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, 
     and rounded to nearest; without them 1.
     """
     return _lib.host().paged_append(xk, xv, k_pages, v_pages, page_table, positions, sequences, xq, freqs,
-                                    layout_code(layout), float(factor), k_scale, v_scale,
-                                    _lib.stream_ptr(xk.device) if xk.is_cuda else 0)
+                                    layout_code(layout), float(factor), k_scale, v_scale)
 
 
 def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -65,5 +64,4 @@ def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, weights are kept to 16 bits; fp32 ones
     are multiplied in fp32.  The same shapes and lengths give the same bits.
     """
-    return _lib.host().paged_attention(xq, k_pages, v_pages, page_table, lengths, scale, k_scale, v_scale, out, lse,
-                                       _lib.stream_ptr(xq.device) if xq.is_cuda else 0)
+    return _lib.host().paged_attention(xq, k_pages, v_pages, page_table, lengths, scale, k_scale, v_scale, out, lse)

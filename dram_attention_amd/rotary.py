@@ -90,37 +90,6 @@ def layout_code(layout: str) -> int:
         raise ValueError(f"layout must be 'interleaved' or 'half' (got {layout!r})") from None
 
 
-def _turn(xq, xk, positions, freqs, half, factor, inverse, in_place):
-    return _lib.host().rotate(xq, xk, positions, freqs, half, factor, inverse, in_place,
-                              _lib.stream_ptr(xq.device) if xq.is_cuda else 0)
-
-
-class _Rotate(torch.autograd.Function):
-    """The gradient of a turn is the turn back of the gradient (the matrix is orthogonal but for the factor, which
-    stays), by the same function, so that it has a gradient itself."""
-
-    @staticmethod
-    def forward(ctx, xq, xk, positions, freqs, half, factor, inverse):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, freqs)
-        ctx.how = half, factor, inverse
-        return _turn(xq, xk, positions, freqs, half, factor, inverse, 0)
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        positions, freqs = ctx.saved_tensors
-        half, factor, inverse = ctx.how
-        gq = gq if ctx.needs_input_grad[0] else None
-        gk = gk if ctx.needs_input_grad[1] else None
-        if gq is None and gk is None:
-            dq = dk = None
-        elif gq is None:
-            (dk, _), dq = _Rotate.apply(gk, None, positions, freqs, half, factor, 1 - inverse), None
-        else:
-            dq, dk = _Rotate.apply(gq, gk, positions, freqs, half, factor, 1 - inverse)
-        return dq, dk, None, None, None, None, None
-
-
 def rotate(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor, *,
            layout: str = "interleaved", factor: float = 1.0):
     """(xq, xk) with the first 2 * len(freqs) channels of every head turned by their token's position; the others are
@@ -132,16 +101,13 @@ def rotate(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, f
     ``factor`` are :func:`rotary_frequencies`'s.  bf16, fp16 or fp32 with any strides; products in fp32, rounded once.
     (A captured backward pass needs leaves that no eager graph still holds, as torch's own operators do.)
     """
-    half, factor = layout_code(layout), float(factor)
     if forward_ad._current_level >= 0:
         raise RuntimeError("rotate has no forward-mode derivative")
-    if torch.is_grad_enabled() and (xq.requires_grad or (xk is not None and xk.requires_grad)):
-        return _Rotate.apply(xq, xk, positions, freqs, half, factor, 0)
-    return _turn(xq, xk, positions, freqs, half, factor, 0, 0)
+    return _lib.host().rotate(xq, xk, positions, freqs, layout_code(layout), float(factor), 0)
 
 
 def rotate_(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, freqs: torch.Tensor, *,
             layout: str = "interleaved", factor: float = 1.0):
     """:func:`rotate` in place, without gradients; returns (xq, xk)."""
-    _turn(xq, xk, positions, freqs, layout_code(layout), float(factor), 0, 1)
+    _lib.host().rotate(xq, xk, positions, freqs, layout_code(layout), float(factor), 1)
     return xq, xk
