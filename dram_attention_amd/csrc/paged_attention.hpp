@@ -519,13 +519,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
     }
     {
       f32x4 st[kSets];
+      const bool next_any = more && first_tile(nxt) < nxt.t1;
       if (any) scores(st);
-      if (more) {
+      if (next_any) {
         publish(nxt.t1, first_tile(nxt), page0);
         load_keys();
       }
       if (any) weigh(st);
-      if (more) {
+      if (next_any) {
         load_values();
         load_query(nxt.b);
         next = page1;
