@@ -467,6 +467,10 @@ PyObject *block_tail(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
 const at::Tensor &plain(PyObject *o, const char *name) {
   const at::Tensor *t = tensor_of(o);
   TORCH_CHECK_TYPE(t != nullptr, name, " must be a plain torch.Tensor (got ", Py_TYPE(o)->tp_name, ")");
+  TORCH_CHECK_VALUE(!t->is_neg() && !t->_is_zerotensor(), name, " is a lazy view: resolve it first");
+  // (the kernels count heads, channels and pages in 32 bits; tokens in 64 or refused by them)
+  for (int64_t d = t->dim() - 2; d < t->dim(); ++d)
+    TORCH_CHECK_VALUE(d < 0 || t->size(d) <= 0x7fffffff, name, " of ", t->sizes(), " is too large");
   return *t;
 }
 const at::Tensor *plain_or_none(PyObject *o, const char *name) { return o == Py_None ? nullptr : &plain(o, name); }

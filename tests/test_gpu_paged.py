@@ -391,6 +391,70 @@ def test_the_same_call_gives_the_same_bits_and_streams_do_not_meet():
         assert all(torch.equal(x, y) for y in ys)
 
 
+def test_two_graphs_of_one_pool_do_not_share_their_workspaces():
+    """Captured calls of unlike shapes, replayed in turn and with eager calls and other allocations between."""
+    g = gen(22)
+    long, _ = attention_case(g, [6000, 900], 8, 2, 128, torch.bfloat16)
+    q, kp, vp, table, lengths = long
+    short = (q[:1].clone(), kp, vp, table[:1], lengths[:1].clone())
+    want = paged_decode_attention(*long), paged_decode_attention(*short)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for args in (long, short):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(paged_decode_attention(*args))
+        graphs.append(graph)
+    for turn in range(4):
+        for i in (turn % 2, 1 - turn % 2):
+            outs[i].fill_(float("nan"))
+            graphs[i].replay()
+            junk = torch.full((1 << 22,), float("nan"), device=DEV)
+            assert torch.equal(paged_decode_attention(*long), want[0])
+            del junk
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1])
+    lengths.fill_(17)           # the lengths are the device's: a replay sees them
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], paged_decode_attention(*long))
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    g = gen(23)
+    cases = [attention_case(g, lengths, 4, 2, 64, torch.bfloat16)[0] for lengths in ([3000], [40] * 30, [700, 2], [1])]
+    want = [paged_decode_attention(*a) for a in cases]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = paged_decode_attention(*cases[i])
+                stream.synchronize()
+                if not torch.equal(got, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_pages_shared_by_sequences():
+    """A common beginning: the same page numbers in several rows of the table."""
+    args, _ = attention_case(gen(24), [320, 64, 1000], 4, 2, 64, torch.float16)
+    q, kp, vp, table, lengths = args
+    table[1, :4] = table[0, :4]
+    table[2, :20] = table[0, :20]
+    check_attention(args, {})
+
+
 # ---- a run of them -------------------------------------------------------------------
 
 @pytest.mark.parametrize("types", [(torch.bfloat16, None), (torch.float32, None), (torch.bfloat16, E4M3)],

@@ -187,6 +187,42 @@ def test_rotating_back_and_forth_through_a_graph_and_on_another_stream():
             assert torch.equal(rotate(ql, kl, positions, freqs)[0], yq)
 
 
+def test_gradients_on_another_stream_and_under_autocast():
+    g = gen(8)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(300, device=DEV)
+    q, gr = randn(g, 300, 4, 64, dtype=torch.bfloat16), randn(g, 300, 4, 64, dtype=torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.autocast("cuda", dtype=torch.float16):
+        leaf = q.clone().requires_grad_()
+        y, _ = rotate(leaf, None, positions, freqs)
+        y.backward(gr)
+    side.synchronize()
+    assert y.dtype == torch.bfloat16
+    check(y, q, positions, freqs, "interleaved")
+    check(leaf.grad, gr, -positions, freqs, "interleaved")
+
+
+def test_positions_changed_before_the_backward_pass_are_noticed():
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(4, device=DEV)
+    x = torch.ones(4, 2, 64, device=DEV, requires_grad=True)
+    y, _ = rotate(x, None, positions, freqs)
+    positions.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_what_is_turned_in_place_is_noticed_by_a_graph_that_needs_it():
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    x, w = torch.ones(4, 2, 64, device=DEV), torch.ones(4, 2, 64, device=DEV, requires_grad=True)
+    y = (x * w).sum()
+    rotate_(x, None, torch.arange(4, device=DEV), freqs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_many_waves():
     """More waves than a grid's first dimension has threads in one workgroup, heads in several windows."""
     T, H, D = 20011, 9, 64

@@ -80,6 +80,23 @@ def test_rotate_refuses(other, kind, match):
         rotate_(**rotate_operands(**other))
 
 
+def test_rotate_refuses_lazy_negatives_and_sizes_that_32_bits_do_not_hold():
+    x = torch.zeros(2, 3, 4, 64, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match="lazy"):
+        rotate(**rotate_operands(xq=x))
+    with pytest.raises(ValueError, match="too large"):
+        rotate(**rotate_operands(xq=torch.zeros(1, 1, 1, 64).expand(2, 3, 2 ** 32 + 4, 64)))
+
+
+def test_rotate_refuses_subclasses():
+    class Kind(torch.Tensor):
+        pass
+
+    with pytest.raises(TypeError, match="plain"):
+        rotate(**rotate_operands(xq=torch.zeros(2, 3, 4, 64).as_subclass(Kind)))
+
+
 def test_rotate_refuses_forward_mode():
     import torch.autograd.forward_ad as fwad
 
