@@ -66,16 +66,38 @@ __device__ __forceinline__ void turn_of(double position, double freq, float fact
   s = factor * sign * (n & 2 ? -s1 : s1);
 }
 
-// A lane's kN elements as they are loaded: a 16-byte vector, or one element.
+template <int kWords>
+struct Words;
+template <>
+struct Words<1> { typedef uint32_t type; };
+template <>
+struct Words<2> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <>
+struct Words<4> { typedef u32x4 type; };
+
+// A lane's kN elements as they are loaded: 16, 8 or 4 bytes, or one element.
 // kStream: rows come and go by streaming loads and stores.
 template <typename T, int kN, bool kStream>
 struct Held {
-  u32x4 v;
+  static constexpr int kWords = kN * T::kBytes / 4;
+  typedef typename Words<kWords>::type Vec;
+  uint32_t w[kWords];
   __device__ __forceinline__ void load(const char *p, int at) {
-    p += (int64_t)at * T::kBytes;
-    v = kStream ? load16_stream(p) : load16(p);
+    const Vec *from = (const Vec *)(p + (int64_t)at * T::kBytes);
+    const Vec v = kStream ? __builtin_nontemporal_load(from) : *from;
+    memcpy(w, &v, sizeof(v));
   }
-  __device__ __forceinline__ void values(float *f) const { unpack<T>(v, f); }
+  __device__ __forceinline__ void values(float *f) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (T::kBytes == 4) {
+        f[i] = as_f32(w[i]);
+      } else {
+        f[2 * i] = __is_same(T, BF16) ? bf16_lo(w[i]) : f16_lo(w[i]);
+        f[2 * i + 1] = __is_same(T, BF16) ? bf16_hi(w[i]) : f16_hi(w[i]);
+      }
+    }
+  }
 };
 template <typename T, bool kStream>
 struct Held<T, 1, kStream> {
@@ -89,27 +111,36 @@ __device__ __forceinline__ void store_row(char *p, int at, float *f, float scale
   if constexpr (TC::kBytes == 1) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) f[i] = f[i] / scale;
-    if constexpr (kN == 8) {
-      uint32_t *d = (uint32_t *)(p + at);
-      *(uint2 *)d = make_uint2(pack_e4m3(f), pack_e4m3(f + 4));
+    if constexpr (kN >= 4) {
+#pragma unroll
+      for (int i = 0; i < kN; i += 4) ((uint32_t *)(p + at))[i / 4] = pack_e4m3(f + i);
     } else {
-      const float one[4] = {f[0], 0.f, 0.f, 0.f};
-      p[at] = (char)pack_e4m3(one);
+      const float some[4] = {f[0], kN == 2 ? f[kN - 1] : 0.f, 0.f, 0.f};
+      const uint32_t w = pack_e4m3(some);
+      if constexpr (kN == 2) *(uint16_t *)(p + at) = (uint16_t)w;
+      else p[at] = (char)w;
     }
   } else if constexpr (kN == 1) {
     store_elem<TC>(p, at, f[0]);
   } else {
-    p += (int64_t)at * TC::kBytes;
-    if constexpr (kStream)
-      store16_stream(p, pack_vec<TC>(f));
-    else
-      store16(p, pack_vec<TC>(f));
+    constexpr int kWords = kN * TC::kBytes / 4;
+    typedef typename Words<kWords>::type Vec;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (TC::kBytes == 4) w[i] = __builtin_bit_cast(uint32_t, f[i]);
+      else w[i] = __is_same(TC, BF16) ? pack_bf16(f[2 * i], f[2 * i + 1]) : pack_f16(f[2 * i], f[2 * i + 1]);
+    }
+    Vec v, *to = (Vec *)(p + (int64_t)at * TC::kBytes);
+    memcpy(&v, w, sizeof(v));
+    if constexpr (kStream) __builtin_nontemporal_store(v, to);
+    else *to = v;
   }
 }
 
-// kN: elements a load (a 16-byte vector, or 1 where a row's parts are no whole vectors).  kPairsInside: the
-// interleaved layout by vectors, whose pairs lie inside one; otherwise an item is the two vectors (or elements) of
-// kN pairs, and behind those single ones that are copied.
+// kN: elements a load, as many as divide a row's parts (16 bytes where they do: a 20-channel turn of heads of 80 takes 4
+// bytes a lane).  kPairsInside: the interleaved layout by vectors, whose pairs lie inside one; otherwise an item is
+// the two vectors (or elements) of kN pairs, and behind those single ones that are copied.
 template <typename T, typename TC, int kN, bool kPairsInside, bool kPaged, bool kStream>
 __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArgs a) {
   __shared__ float2 turns[kMaxTurns];
@@ -229,15 +260,13 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
   }
 }
 
-static bool multiple(int64_t v, int of) { return v % of == 0; }
-
 // Workgroups that fill the chip; tokens are taken several at a time where there are more.
 constexpr int kTurnGrid = 1024;
 
-// Fills what follows from the shape; rows of whole 16-byte vectors (`vectors`) or element by element.
-static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool vectors, const char *what) {
-  const int n = vectors ? vec : 1, pairs = a.rotary_dim / 2;
-  const bool inside = vectors && !a.half;
+// Fills what follows from the shape, rows taken `n` elements a load.
+static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int n, const char *what) {
+  const int pairs = a.rotary_dim / 2;
+  const bool inside = n > 1 && !a.half;
   a.cols = inside ? a.head_dim / n : pairs / n + (a.head_dim - a.rotary_dim) / n;
   a.lanes_shift = 0;
   while (a.lanes_shift < 6 && (1 << a.lanes_shift) < a.cols) ++a.lanes_shift;
@@ -262,17 +291,23 @@ static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int vec, bool 
 constexpr int64_t kStreamBytes = (int64_t)256 << 20;
 
 template <typename T, typename TC, bool kPaged>
-static int launch_rows(const TurnArgs &a, bool vectors, hipStream_t s, const char *what) {
+static int launch_rows(const TurnArgs &a, int n, hipStream_t s, const char *what) {
   const dim3 grid((unsigned)ceil_div(a.tokens, a.group)), block(kTurnThreads);
   const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
   const bool stream = rows * a.tokens * a.head_dim * 2 * T::kBytes >= kStreamBytes;
 #define DA_TURN(n, inside, streaming) \
   hipLaunchKernelGGL((rotary_rows_kernel<T, TC, n, inside, kPaged, streaming>), grid, block, 0, s, a)
-  if (!vectors) DA_TURN(1, false, false);
-  else if (a.half && stream) DA_TURN(T::kVec, false, true);
-  else if (a.half) DA_TURN(T::kVec, false, false);
-  else if (stream) DA_TURN(T::kVec, true, true);
-  else DA_TURN(T::kVec, true, false);
+#define DA_TURN_LAYOUT(n, streaming)   \
+  do {                                 \
+    if (a.half) DA_TURN(n, false, streaming); \
+    else DA_TURN(n, true, streaming);  \
+  } while (0)
+  if (n == T::kVec && stream) DA_TURN_LAYOUT(T::kVec, true);
+  else if (n == T::kVec) DA_TURN_LAYOUT(T::kVec, false);
+  else if (n == T::kVec / 2) DA_TURN_LAYOUT(T::kVec / 2, false);
+  else if (n == 2) DA_TURN_LAYOUT(2, false);
+  else DA_TURN(1, false, false);
+#undef DA_TURN_LAYOUT
 #undef DA_TURN
   return launch_status(what);
 }
@@ -287,9 +322,11 @@ static int check_turn(int head_dim, int rotary_dim, int layout, int dtype, const
     return fail(DA_ENOTSUP, "%s: up to %d channels that turn, heads of up to 65536", what, 2 * kMaxPairs);
   return DA_OK;
 }
-// Whether a turned row's parts are whole vectors of `vec` elements.
-static bool whole_vectors(int head_dim, int rotary_dim, int half, int vec) {
-  return multiple(head_dim, vec) && multiple(half ? rotary_dim / 2 : rotary_dim, vec);
+// The most elements a load, at most 16 bytes and a power of two, that divide everything in `parts` (elements).
+static int elements_a_load(int vec, int64_t parts) {
+  int n = vec;
+  while (n > 1 && parts % n != 0) n /= 2;
+  return n;
 }
 
 }  // namespace da
@@ -315,26 +352,29 @@ extern "C" int da_rotate(const void *args, size_t args_bytes, void *stream) {
   void *y[2] = {r.q_out, r.k_out};
   const int64_t *xs[2] = {r.q_strides, r.k_strides}, *ys[2] = {r.q_out_strides, r.k_out_strides};
   const int32_t heads[2] = {r.n_q_heads, r.n_k_heads};
-  bool vectors = whole_vectors(r.head_dim, r.rotary_dim, r.layout, vec);
+  // (what all offsets have in common is the lowest bit of their union)
+  int64_t parts = r.head_dim | (r.layout ? r.rotary_dim / 2 : r.rotary_dim);
   for (int i = 0; i < 2; ++i) {
     a.x[i] = (const char *)x[i];
     a.y[i] = (char *)y[i];
     a.x_batch_b[i] = xs[i][0] * e, a.x_tok_b[i] = xs[i][1] * e, a.x_head_b[i] = xs[i][2] * e;
     a.y_batch_b[i] = ys[i][0] * e, a.y_tok_b[i] = ys[i][1] * e, a.y_head_b[i] = ys[i][2] * e;
     if (!heads[i]) continue;
-    vectors = vectors && multiple((uintptr_t)x[i] | (uintptr_t)y[i], 16);
-    for (int j = 0; j < 3; ++j) vectors = vectors && multiple(xs[i][j], vec) && multiple(ys[i][j], vec);
+    DA_REQUIRE(((uintptr_t)x[i] | (uintptr_t)y[i]) % e == 0, "da_rotate: rows must be aligned to their elements");
+    parts |= (int64_t)(((uintptr_t)x[i] | (uintptr_t)y[i]) / e);
+    for (int j = 0; j < 3; ++j) parts |= xs[i][j] | ys[i][j];
   }
+  const int n = elements_a_load(vec, parts);
   a.rows[0] = r.n_q_heads, a.rows[1] = r.n_k_heads;
   a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
   a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type;
   a.pos_batch_stride = r.position_strides[0], a.pos_tok_stride = r.position_strides[1];
   a.factor = r.factor, a.sign = r.inverse ? -1.f : 1.f;
-  if (int rc = shape_rows(a, r.batch, r.tokens, vec, vectors, "da_rotate")) return rc;
+  if (int rc = shape_rows(a, r.batch, r.tokens, n, "da_rotate")) return rc;
   hipStream_t s = (hipStream_t)stream;
-  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, false>(a, vectors, s, "da_rotate");
-  if (r.dtype == DA_F16) return launch_rows<F16, F16, false>(a, vectors, s, "da_rotate");
-  return launch_rows<F32, F32, false>(a, vectors, s, "da_rotate");
+  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, false>(a, n, s, "da_rotate");
+  if (r.dtype == DA_F16) return launch_rows<F16, F16, false>(a, n, s, "da_rotate");
+  return launch_rows<F32, F32, false>(a, n, s, "da_rotate");
 }
 
 extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream) {
@@ -367,7 +407,7 @@ extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream
   const void *x[3] = {r.q, r.k, r.v};
   void *y[3] = {r.q_out, r.k_pages, r.v_pages};
   const int64_t *xs[3] = {r.q_strides, r.k_strides, r.v_strides};
-  bool vectors = whole_vectors(r.head_dim, r.rotary_dim, r.layout, vec);
+  int64_t parts = r.head_dim | (r.layout ? r.rotary_dim / 2 : r.rotary_dim);
   for (int i = 0; i < 3; ++i) {
     a.x[i] = (const char *)x[i];
     a.y[i] = (char *)y[i];
@@ -375,15 +415,18 @@ extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream
     if (i == 0) {
       a.y_tok_b[0] = r.q_out_strides[0] * e, a.y_head_b[0] = r.q_out_strides[1] * e;
       if (!r.n_q_heads) continue;
-      vectors = vectors && multiple((uintptr_t)y[0], 16) && multiple(r.q_out_strides[0], vec) &&
-                multiple(r.q_out_strides[1], vec);
+      DA_REQUIRE((uintptr_t)y[0] % e == 0, "da_paged_append: rows must be aligned to their elements");
+      parts |= (int64_t)((uintptr_t)y[0] / e) | r.q_out_strides[0] | r.q_out_strides[1];
     } else {
       a.y_batch_b[i] = r.page_strides[0] * c, a.y_tok_b[i] = r.page_strides[1] * c, a.y_head_b[i] = r.page_strides[2] * c;
-      vectors = vectors && multiple((uintptr_t)y[i], vec * c);
-      for (int j = 0; j < 3; ++j) vectors = vectors && multiple(r.page_strides[j], vec);
+      DA_REQUIRE((uintptr_t)y[i] % c == 0, "da_paged_append: rows must be aligned to their elements");
+      parts |= (int64_t)((uintptr_t)y[i] / c);
+      for (int j = 0; j < 3; ++j) parts |= r.page_strides[j];
     }
-    vectors = vectors && multiple((uintptr_t)x[i], 16) && multiple(xs[i][0], vec) && multiple(xs[i][1], vec);
+    DA_REQUIRE((uintptr_t)x[i] % e == 0, "da_paged_append: rows must be aligned to their elements");
+    parts |= (int64_t)((uintptr_t)x[i] / e) | xs[i][0] | xs[i][1];
   }
+  const int n = elements_a_load(vec, parts);
   a.rows[0] = r.n_q_heads, a.rows[1] = a.rows[2] = r.n_kv_heads;
   a.head_dim = r.head_dim, a.rotary_dim = r.rotary_dim, a.half = r.layout;
   a.freqs = r.freqs, a.positions = r.positions, a.positions64 = r.position_type, a.pos_tok_stride = 1;
@@ -393,13 +436,13 @@ extern "C" int da_paged_append(const void *args, size_t args_bytes, void *stream
   a.n_sequences = r.n_sequences, a.n_pages = r.n_pages, a.max_tokens = (int32_t)room;
   a.by_page = divisor_of(r.page_size);
   a.scale[1] = r.k_scale, a.scale[2] = r.v_scale;
-  if (int rc = shape_rows(a, 1, r.n_tokens, vec, vectors, "da_paged_append")) return rc;
+  if (int rc = shape_rows(a, 1, r.n_tokens, n, "da_paged_append")) return rc;
   hipStream_t s = (hipStream_t)stream;
   if (r.page_dtype == DA_E4M3) {
-    if (r.dtype == DA_BF16) return launch_rows<BF16, E4M3, true>(a, vectors, s, "da_paged_append");
-    return launch_rows<F16, E4M3, true>(a, vectors, s, "da_paged_append");
+    if (r.dtype == DA_BF16) return launch_rows<BF16, E4M3, true>(a, n, s, "da_paged_append");
+    return launch_rows<F16, E4M3, true>(a, n, s, "da_paged_append");
   }
-  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, true>(a, vectors, s, "da_paged_append");
-  if (r.dtype == DA_F16) return launch_rows<F16, F16, true>(a, vectors, s, "da_paged_append");
-  return launch_rows<F32, F32, true>(a, vectors, s, "da_paged_append");
+  if (r.dtype == DA_BF16) return launch_rows<BF16, BF16, true>(a, n, s, "da_paged_append");
+  if (r.dtype == DA_F16) return launch_rows<F16, F16, true>(a, n, s, "da_paged_append");
+  return launch_rows<F32, F32, true>(a, n, s, "da_paged_append");
 }

@@ -56,6 +56,11 @@ CASES = [   # dtype, cache, kv heads, heads, head_dim, page, rotary, layout, poo
     (torch.float32, None, 2, 8, 64, 16, 64, "interleaved", "pages"),
     (torch.float32, None, 2, 2, 5, 3, 4, "half", "rows"),
     (torch.bfloat16, None, 5, 0, 256, 100, 64, "half", "pages"),
+    # (rows taken 4 and 2 elements a load)
+    (torch.float16, E4M3, 3, 3, 96, 16, 24, "half", "pages"),
+    (torch.bfloat16, E4M3, 2, 4, 80, 16, 20, "half", "rows"),
+    (torch.bfloat16, None, 2, 4, 80, 16, 20, "interleaved", "pages"),
+    (torch.float32, None, 2, 4, 80, 16, 20, "half", "pages"),
 ]
 
 

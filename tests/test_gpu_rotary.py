@@ -29,7 +29,7 @@ def check(got, x, positions, freqs, layout, factor=1.0):
 # (tokens, heads, kv heads, head_dim, rotary_dim)
 SHAPES = [(1, 32, 8, 128, 128), (1, 1, 1, 8, 2), (257, 5, 3, 80, 20), (64, 7, 1, 64, 64), (33, 4, 2, 128, 32),
           (19, 3, 3, 96, 96), (10, 2, 1, 256, 256), (5, 3, 1, 512, 512), (9, 2, 2, 66, 66), (7, 40, 2, 24, 8),
-          (3, 2, 1, 5, 4), (300, 70, 10, 16, 16)]
+          (3, 2, 1, 5, 4), (300, 70, 10, 16, 16), (65, 4, 1, 96, 24), (31, 3, 2, 20, 12)]
 
 
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
