@@ -11,10 +11,10 @@
 // the millionth position of the fastest pair.  Whole turns go away in 64 bits, then quarters of a turn, and sine and
 // cosine of the rest are Taylor polynomials on |t| <= pi/4 (their next terms are below 2^-26).
 //
-// Bound: HBM; a row is read once and written once, 16 bytes a lane.  A workgroup takes a few tokens: its threads form
-// their angles, about one pair each, into LDS, while the first rows are on their way.  Its waves then take blocks of as
-// many head rows as 64 lanes hold, kInFlight blocks at a time; which token, tensor and rows a block is, is the same for
-// the whole wave and left to the scalar unit.
+// Bound: HBM; a row is read once and written once, up to 16 bytes a lane.  A workgroup takes a few tokens: its threads
+// form their angles, about one pair each, into LDS, while the first rows are on their way.  Its waves then take blocks of
+// 64 items (a load and a store each) of a token's head rows laid end to end, kInFlight blocks at a time; which token,
+// tensor and block it is, is the same for the whole wave and left to the scalar unit.
 #include "paged_math.hpp"
 
 namespace da {
@@ -32,8 +32,9 @@ struct TurnArgs {
   int64_t x_batch_b[3], x_tok_b[3], x_head_b[3];
   int64_t y_batch_b[3], y_tok_b[3], y_head_b[3];   // (y of k and v in pages: page, token, head)
   int32_t rows[3];                                 // heads
-  int32_t block_end[3];                            // a token's blocks up to and with q's, k's, v's
-  int32_t cols, lanes_shift;                       // items of a row; lanes that take them, as a power of two
+  int32_t items[3];                                // of a token
+  int32_t block_end[3];                            // a token's blocks of 64 items up to and with q's, k's, v's
+  Divisor by_cols;                                 // items of a row
   int32_t head_dim, rotary_dim, half;
   int32_t tokens, group;                           // of all batches; of a workgroup
   Divisor by_tokens, by_blocks, by_pairs;          // tokens of a batch, blocks of a token, pairs of a row
@@ -148,8 +149,6 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int first = (int)blockIdx.x * a.group, count = min(a.group, a.tokens - first);
   const int pairs = a.rotary_dim / 2;
-  const int lanes = 1 << a.lanes_shift, rows_per_block = 64 >> a.lanes_shift;
-  const int row0 = lane >> a.lanes_shift, col0 = lane & (lanes - 1);
   const int turned_cols = kPairsInside ? a.rotary_dim / kN : pairs / kN;
   const int blocks = a.by_blocks.d * count;
 
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
 
   // What a block is (the same for the wave's lanes).
   struct Block {
-    int tok, w, row;   // within the workgroup's tokens; tensor; first row
+    int tok, w, item;   // within the workgroup's tokens; tensor; first item
     int64_t batch, in_batch;
   };
   auto block_at = [&](int j) {
@@ -171,22 +170,22 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
     x.tok = divide(j, a.by_blocks);
     const int within = j - x.tok * a.by_blocks.d;
     x.w = within < a.block_end[0] ? 0 : !kPaged || within < a.block_end[1] ? 1 : 2;
-    x.row = (within - (x.w ? a.block_end[x.w - 1] : 0)) * rows_per_block;
+    x.item = (within - (x.w ? a.block_end[x.w - 1] : 0)) * 64;
     x.batch = divide(first + x.tok, a.by_tokens);
     x.in_batch = first + x.tok - (int)x.batch * a.by_tokens.d;
     return x;
   };
   Held<T, kN, kStream> ha[kInFlight], hb[kInFlight];
-  auto load = [&](const Block &x, int col, int u) {
-    const int row = x.row + row0;
-    if (row >= a.rows[x.w] || col >= a.cols) return;
+  auto load = [&](const Block &x, int u) {
+    const int item = x.item + lane, row = divide(item, a.by_cols), col = item - row * a.by_cols.d;
+    if (item >= a.items[x.w]) return;
     const char *p = a.x[x.w] + x.batch * a.x_batch_b[x.w] + x.in_batch * a.x_tok_b[x.w] + row * a.x_head_b[x.w];
     ha[u].load(p, at_a(col));
     if (!kPairsInside && col < turned_cols) hb[u].load(p, at_b(col));
   };
-  auto store = [&](const Block &x, int col, int u) {
-    const int row = x.row + row0;
-    if (row >= a.rows[x.w] || col >= a.cols) return;
+  auto store = [&](const Block &x, int u) {
+    const int item = x.item + lane, row = divide(item, a.by_cols), col = item - row * a.by_cols.d;
+    if (item >= a.items[x.w]) return;
     float fa[kN], fb[kN];
     const bool paired = !kPairsInside && col < turned_cols;
     ha[u].values(fa);
@@ -216,47 +215,44 @@ __global__ void __launch_bounds__(kTurnThreads) rotary_rows_kernel(const TurnArg
   };
 
   bool formed = false;
-  for (int base = 0; base < a.cols; base += lanes) {   // rows wider than 64 items go in steps of 64
-    const int col = base + col0;
-    // (a wave without a block still has angles to form and a barrier to reach)
-    for (int j0 = wave; j0 < blocks || !formed; j0 += kInFlight * kTurnWaves) {
+  // (a wave without a block still has angles to form and a barrier to reach)
+  for (int j0 = wave; j0 < blocks || !formed; j0 += kInFlight * kTurnWaves) {
 #pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (j0 + u * kTurnWaves < blocks) load(block_at(j0 + u * kTurnWaves), col, u);
-      if (!formed) {
-        formed = true;
-        auto position = [&](int tok) {
-          const int64_t batch = divide(first + tok, a.by_tokens);
-          return load_index(a.positions, a.positions64,
-                            batch * a.pos_batch_stride + (first + tok - (int)batch * a.by_tokens.d) * a.pos_tok_stride);
-        };
-        for (int i = threadIdx.x; i < count * pairs; i += kTurnThreads) {
-          const int tok = divide(i, a.by_pairs);
-          float c, s;
-          turn_of((double)position(tok), a.freqs[i - tok * pairs], a.factor, a.sign, c, s);
-          turns[i] = make_float2(c, s);
-        }
-        if constexpr (kPaged) {
-          if (threadIdx.x < count) {
-            const int64_t pos = position(threadIdx.x);
-            const int64_t seq = a.sequences ? load_index(a.sequences, a.sequences64, first + threadIdx.x)
-                                            : (int64_t)(first + threadIdx.x);
-            int64_t place = -1;
-            if (seq >= 0 && seq < a.n_sequences && pos >= 0 && pos < a.max_tokens) {
-              const int page = divide((int)pos, a.by_page);
-              const int64_t number = load_index(a.table, a.table64, seq * a.table_stride + page);
-              if (number >= 0 && number < a.n_pages)
-                place = number * a.y_batch_b[1] + (int64_t)((int)pos - page * a.by_page.d) * a.y_tok_b[1];
-            }
-            places[threadIdx.x] = place;
-          }
-        }
-        __syncthreads();
+    for (int u = 0; u < kInFlight; ++u)
+      if (j0 + u * kTurnWaves < blocks) load(block_at(j0 + u * kTurnWaves), u);
+    if (!formed) {
+      formed = true;
+      auto position = [&](int tok) {
+        const int64_t batch = divide(first + tok, a.by_tokens);
+        return load_index(a.positions, a.positions64,
+                          batch * a.pos_batch_stride + (first + tok - (int)batch * a.by_tokens.d) * a.pos_tok_stride);
+      };
+      for (int i = threadIdx.x; i < count * pairs; i += kTurnThreads) {
+        const int tok = divide(i, a.by_pairs);
+        float c, s;
+        turn_of((double)position(tok), a.freqs[i - tok * pairs], a.factor, a.sign, c, s);
+        turns[i] = make_float2(c, s);
       }
-#pragma unroll
-      for (int u = 0; u < kInFlight; ++u)
-        if (j0 + u * kTurnWaves < blocks) store(block_at(j0 + u * kTurnWaves), col, u);
+      if constexpr (kPaged) {
+        if (threadIdx.x < count) {
+          const int64_t pos = position(threadIdx.x);
+          const int64_t seq = a.sequences ? load_index(a.sequences, a.sequences64, first + threadIdx.x)
+                                          : (int64_t)(first + threadIdx.x);
+          int64_t place = -1;
+          if (seq >= 0 && seq < a.n_sequences && pos >= 0 && pos < a.max_tokens) {
+            const int page = divide((int)pos, a.by_page);
+            const int64_t number = load_index(a.table, a.table64, seq * a.table_stride + page);
+            if (number >= 0 && number < a.n_pages)
+              place = number * a.y_batch_b[1] + (int64_t)((int)pos - page * a.by_page.d) * a.y_tok_b[1];
+          }
+          places[threadIdx.x] = place;
+        }
+      }
+      __syncthreads();
     }
+#pragma unroll
+    for (int u = 0; u < kInFlight; ++u)
+      if (j0 + u * kTurnWaves < blocks) store(block_at(j0 + u * kTurnWaves), u);
   }
 }
 
@@ -267,11 +263,15 @@ constexpr int kTurnGrid = 1024;
 static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int n, const char *what) {
   const int pairs = a.rotary_dim / 2;
   const bool inside = n > 1 && !a.half;
-  a.cols = inside ? a.head_dim / n : pairs / n + (a.head_dim - a.rotary_dim) / n;
-  a.lanes_shift = 0;
-  while (a.lanes_shift < 6 && (1 << a.lanes_shift) < a.cols) ++a.lanes_shift;
+  const int cols = inside ? a.head_dim / n : pairs / n + (a.head_dim - a.rotary_dim) / n;
+  a.by_cols = divisor_of(cols);
   int64_t blocks = 0;
-  for (int i = 0; i < 3; ++i) a.block_end[i] = (int32_t)(blocks += ceil_div(a.rows[i], 64 >> a.lanes_shift));
+  for (int i = 0; i < 3; ++i) {
+    const int64_t items = (int64_t)a.rows[i] * cols;
+    blocks += ceil_div(items, 64);
+    if (blocks > 1 << 24) return fail(DA_ENOTSUP, "%s: %d heads of %d channels are too many", what, a.rows[i], a.head_dim);
+    a.items[i] = (int32_t)items, a.block_end[i] = (int32_t)blocks;
+  }
   if (tokens > 0x7fffff00 / batch)   // (counted in 32 bits, a workgroup's tokens ahead)
     return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens are too many", what, (long long)batch, (long long)tokens);
   a.tokens = (int32_t)(batch * tokens);
