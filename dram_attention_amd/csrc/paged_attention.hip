@@ -14,7 +14,7 @@ constexpr int kPagedDirect = 512, kPagedDirectMany = 1024;
 constexpr int64_t kPagedMostTokens = (int64_t)1 << 30;   // of a sequence: tiles ahead are counted in 32 bits
 
 struct PagedPlan {
-  int32_t groups, shares;
+  int32_t groups, group_rows, shares;
   size_t prefix_bytes, ml_bytes, acc_bytes;
   size_t bytes() const { return shares > 1 ? prefix_bytes + ml_bytes + acc_bytes : 0; }
 };
@@ -24,17 +24,19 @@ static int64_t paged_room(const da_paged_attention_args &r) { return (int64_t)r.
 static PagedPlan paged_plan(const da_paged_attention_args &r) {
   PagedPlan p = {};
   const int rep = r.n_q_heads / r.n_kv_heads;
-  p.groups = (int32_t)ceil_div(rep, 16);
+  const int sixteens = paged_sixteens(r.head_dim, elem_size(r.dtype), rep);
+  p.group_rows = 16 * sixteens;
+  p.groups = (int32_t)ceil_div(rep, p.group_rows);
   const int64_t head_groups = (int64_t)r.n_kv_heads * p.groups;
   const int64_t room = paged_room(r), units = ceil_div(room, r.dtype == DA_F32 ? 64 : 128);
   const int bytes = r.page_dtype == DA_E4M3 ? 1 : elem_size(r.dtype);
-  int64_t shares = kComputeUnits * paged_resident(r.head_dim, bytes) / head_groups;
+  int64_t shares = kComputeUnits * paged_resident(r.head_dim, bytes, sixteens) / head_groups;
   if (shares > units * r.n_sequences) shares = units * r.n_sequences;
   const bool many = r.n_sequences * head_groups >= 2 * kComputeUnits;
   if (room <= (many ? kPagedDirectMany : kPagedDirect) || shares <= 1) return p;
-  static_assert(kComputeUnits * paged_resident(64, 1) <= kPagedMostShares, "the join's threads hold that many");
+  static_assert(kComputeUnits * paged_resident(64, 1, 1) <= kPagedMostShares, "the join's threads hold that many");
   p.shares = (int32_t)shares;
-  const int64_t rows = head_groups * shares * 2 * 16;
+  const int64_t rows = head_groups * shares * 2 * p.group_rows;
   p.prefix_bytes = (size_t)ceil_div(((int64_t)r.n_sequences + 1) * 4, 16) * 16;
   p.ml_bytes = (size_t)rows * 2 * 4;
   p.acc_bytes = (size_t)rows * r.head_dim * 4;
@@ -105,7 +107,7 @@ extern "C" int da_paged_attention(const void *args, size_t args_bytes, void *str
   a.lengths = r.lengths, a.lengths64 = r.length_type;
   a.n_seqs = r.n_sequences, a.n_pages = r.n_pages, a.max_tokens = most;
   a.by_page = divisor_of(r.page_size);
-  a.n_q_heads = r.n_q_heads, a.n_kv_heads = r.n_kv_heads, a.rep = r.n_q_heads / r.n_kv_heads, a.groups = plan.groups;
+  a.n_q_heads = r.n_q_heads, a.n_kv_heads = r.n_kv_heads, a.rep = r.n_q_heads / r.n_kv_heads, a.groups = plan.groups, a.group_rows = plan.group_rows;
   a.shares = plan.shares;
   a.scale_log2 = r.scale * kLog2e;
   a.k_scale = r.k_scale, a.v_scale = r.v_scale;

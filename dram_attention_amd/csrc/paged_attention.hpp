@@ -35,10 +35,17 @@ constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kPagedMostShares = 1024;
 constexpr int kDies = 8;
 
-// Workgroups that a compute unit holds.
-constexpr int paged_resident(int head_dim, int bytes) {
-  return head_dim == 64 ? 4 : head_dim == 96 || (head_dim == 128 && bytes == 1) ? 3 : head_dim == 128 || bytes == 1 ? 2 : 1;
+// Workgroups that a compute unit holds, by the registers that `sixteens` of query rows take.
+constexpr int paged_resident(int head_dim, int bytes, int sixteens) {
+  return sixteens > 1     ? (head_dim == 64 ? 3 : 2)
+         : head_dim == 64 ? 4
+         : head_dim == 96 || (head_dim == 128 && bytes == 1) ? 3
+         : head_dim == 128 || bytes == 1                     ? 2
+                                                             : 1;
 }
+// Sixteens of query rows that share a wave's keys and values, where a kv head has more: 64/2 heads over 1 GB 176 us
+// instead of 216 as two workgroups, 64/1 234 instead of 354.
+constexpr int paged_sixteens(int head_dim, int bytes, int rep) { return rep > 16 && head_dim <= 128 && bytes < 4 ? 2 : 1; }
 
 struct PagedArgs {
   const char *q, *k, *v;
@@ -48,7 +55,8 @@ struct PagedArgs {
   int32_t table64, lengths64;
   int32_t n_seqs, n_pages, max_tokens;
   Divisor by_page;
-  int32_t n_q_heads, n_kv_heads, rep, groups;   // groups: of 16 query rows, of a kv head
+  int32_t n_q_heads, n_kv_heads, rep;
+  int32_t groups, group_rows;                   // groups of 16 or 32 query rows of a kv head
   int32_t shares;                               // 0: a workgroup per sequence, nothing is joined
   float scale_log2;
   const float *k_scale, *v_scale;
@@ -173,8 +181,9 @@ __device__ __forceinline__ void write_sums(const PagedArgs &a, bool whole, int64
   }
 }
 
-template <typename T, typename KV, int kD, bool kStream>
-__global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes)) paged_attention_kernel(const PagedArgs a) {
+// kM: sixteens of query rows that share the keys and values a wave holds.
+template <typename T, typename KV, int kD, bool kStream, int kM>
+__global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, kM)) paged_attention_kernel(const PagedArgs a) {
   using Tile = PagedTile<T, KV, kD>;
   constexpr bool kWide = Tile::kWide;
   constexpr int kSets = Tile::kSets, kTokens = Tile::kTokens, kUnit = Tile::kUnit, kSteps = Tile::kSteps;
@@ -197,8 +206,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
   const int width = min(kDies, line - turn * kDies), group = in_turn / width;
   const int at_line = turn * kDies + in_turn - group * width;
   const int share = at_line / a.n_kv_heads, h = at_line - share * a.n_kv_heads, hg = h * a.groups + group;
-  const int rows = a.rep - 16 * group < 16 ? a.rep - 16 * group : 16;
-  const int64_t first_q = (int64_t)h * a.rep + 16 * group;
+  const int rows = min(a.rep - 16 * kM * group, 16 * kM);
+  const int64_t first_q = (int64_t)h * a.rep + 16 * kM * group;
   const float scale_log2 = a.scale_log2 * (KV::kBytes == 1 && a.k_scale ? a.k_scale[h] : 1.f);
   const float v_scale = KV::kBytes == 1 && a.v_scale ? a.v_scale[h] : 1.f;
 
@@ -289,18 +298,22 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
     }
     return x;
   };
-  u32x4 qv[kSteps];
+  u32x4 qv[kM][kSteps];
   auto load_query = [&](int b) {
-    const char *qp = a.q + b * a.q_seq_b + (first_q + (c < rows ? c : 0)) * a.q_head_b;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      qv[s] = load16(qp + Tile::piece(s, g) * T::kBytes);
-      if (c >= rows) qv[s] = u32x4{0, 0, 0, 0};
+    for (int r = 0; r < kM; ++r) {
+      const int row = 16 * r + c;
+      const char *qp = a.q + b * a.q_seq_b + (first_q + (row < rows ? row : 0)) * a.q_head_b;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        qv[r][s] = load16(qp + Tile::piece(s, g) * T::kBytes);
+        if (row >= rows) qv[r][s] = u32x4{0, 0, 0, 0};
+      }
     }
   };
 
-  float m, l;
-  f32x4 acc[kSlice];
+  float m[kM], l[kM];
+  f32x4 acc[kM][kSlice];
   uint32_t kk[kSets][kRowWords];
   uint32_t vv[kHeld][kSliceWords];
   uint32_t live = 0;   // of the tokens held: which count
@@ -373,16 +386,20 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
   };
 
   // S^T of the tile in kk
-  auto scores = [&](f32x4 *st) {
+  auto scores = [&](f32x4 (*st)[kSets]) {
 #pragma unroll
     for (int s = 0; s < kSets; ++s) {
-      f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+      f32x4 x[kM], y[kM];   // two chains
+#pragma unroll
+      for (int r = 0; r < kM; ++r) x[r] = y[r] = f32x4{0.f, 0.f, 0.f, 0.f};
       if constexpr (kWide) {
 #pragma unroll
-        for (int i = 0; i < 4 * kSteps; ++i) {   // two chains
-          f32x4 &z = i & 1 ? y : x;
-          z = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(kk[s][i]), as_f32(qv[i / 4][i % 4]), z, 0, 0, 0);
-        }
+        for (int i = 0; i < 4 * kSteps; ++i)
+#pragma unroll
+          for (int r = 0; r < kM; ++r) {
+            f32x4 &z = i & 1 ? y[r] : x[r];
+            z = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(kk[s][i]), as_f32(qv[r][i / 4][i % 4]), z, 0, 0, 0);
+          }
       } else {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -394,38 +411,45 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
           } else {
             ka = u32x4{kk[s][4 * i], kk[s][4 * i + 1], kk[s][4 * i + 2], kk[s][4 * i + 3]};
           }
-          f32x4 &z = i & 1 ? y : x;
-          z = MatrixOps<T>::k32(ka, qv[i], z);
+#pragma unroll
+          for (int r = 0; r < kM; ++r) {
+            f32x4 &z = i & 1 ? y[r] : x[r];
+            z = MatrixOps<T>::k32(ka, qv[r][i], z);
+          }
         }
       }
-      st[s] = x + y;
+#pragma unroll
+      for (int r = 0; r < kM; ++r) st[r][s] = x[r] + y[r];
     }
   };
 
   // Weights of the tile's scores; O^T += V^T P^T
-  auto weigh = [&](const f32x4 *st) {
-    float p[kHeld];
-    float top = -INFINITY;
+  auto weigh = [&](f32x4 (*st)[kSets]) {
+    float p[kM][kHeld];
 #pragma unroll
-    for (int x = 0; x < kHeld; ++x) {
-      p[x] = live >> x & 1 ? st[x / 4][x % 4] * scale_log2 : -INFINITY;
-      top = fmaxf(top, p[x]);
-    }
-    if (__any(top > m + (Range::kSlack + Range::kBias))) {   // rare
-      float mx = top - Range::kBias;
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m);
-      const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m - mx);
-      m = mx;
-      l *= alpha;
+    for (int r = 0; r < kM; ++r) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < kSlice; ++j) acc[j] *= alpha;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
+      for (int x = 0; x < kHeld; ++x) {
+        p[r][x] = live >> x & 1 ? st[r][x / 4][x % 4] * scale_log2 : -INFINITY;
+        top = fmaxf(top, p[r][x]);
+      }
+      if (__any(top > m[r] + (Range::kSlack + Range::kBias))) {   // rare
+        float mx = top - Range::kBias;
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[r]);
+        const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m[r] - mx);
+        m[r] = mx;
+        l[r] *= alpha;
 #pragma unroll
-    for (int x = 0; x < kHeld; ++x) {
-      p[x] = fast_exp2(p[x] - ref);
-      l += p[x];
+        for (int j = 0; j < kSlice; ++j) acc[r][j] *= alpha;
+      }
+      const float ref = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int x = 0; x < kHeld; ++x) {
+        p[r][x] = fast_exp2(p[r][x] - ref);
+        l[r] += p[r][x];
+      }
     }
     // values of tokens that do not count are memory nobody vouches for: 0 * NaN must not arise
     if (__any(live != (1u << kHeld) - 1)) {
@@ -439,37 +463,41 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
       for (int x = 0; x < kHeld; ++x)
 #pragma unroll
         for (int j = 0; j < kSlice; ++j)
-          acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[x], acc[j], 0, 0, 0);
-    } else {
 #pragma unroll
-      for (int x0 = 0; x0 < kHeld; x0 += 8) {   // eight tokens of the lane at a time
-        u32x4 p1, p2;
+          for (int r = 0; r < kM; ++r)
+            acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[r][x], acc[r][j], 0, 0, 0);
+    } else {
+      u32x4 p1[kM], p2[kM];
+#pragma unroll
+      for (int r = 0; r < kM; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t first, rest;
-          split_weights<T>(p[x0 + 2 * i], p[x0 + 2 * i + 1], first, rest);
-          p1[i] = first, p2[i] = rest;
+          split_weights<T>(p[r][2 * i], p[r][2 * i + 1], first, rest);
+          p1[r][i] = first, p2[r][i] = rest;
         }
 #pragma unroll
-        for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
-          uint32_t w[8];
+      for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
+        uint32_t w[8];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            if constexpr (KV::kBytes == 1)
-              w[x] = jj & 1 ? widen_e4m3<T, true>(vv[x0 + x][jj / 2]) : widen_e4m3<T, false>(vv[x0 + x][jj / 2]);
-            else
-              w[x] = vv[x0 + x][jj];
-          }
-          u32x4 even, odd;
+        for (int x = 0; x < 8; ++x) {
+          if constexpr (KV::kBytes == 1)
+            w[x] = jj & 1 ? widen_e4m3<T, true>(vv[x][jj / 2]) : widen_e4m3<T, false>(vv[x][jj / 2]);
+          else
+            w[x] = vv[x][jj];
+        }
+        u32x4 even, odd;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
-            odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
-          }
-          acc[2 * jj] = MatrixOps<T>::k32(even, p1, acc[2 * jj]);
-          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p1, acc[2 * jj + 1]);
-          acc[2 * jj] = MatrixOps<T>::k32(even, p2, acc[2 * jj]);
-          acc[2 * jj + 1] = MatrixOps<T>::k32(odd, p2, acc[2 * jj + 1]);
+        for (int i = 0; i < 4; ++i) {
+          even[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
+          odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
+        }
+#pragma unroll
+        for (int r = 0; r < kM; ++r) {
+          acc[r][2 * jj] = MatrixOps<T>::k32(even, p1[r], acc[r][2 * jj]);
+          acc[r][2 * jj + 1] = MatrixOps<T>::k32(odd, p1[r], acc[r][2 * jj + 1]);
+          acc[r][2 * jj] = MatrixOps<T>::k32(even, p2[r], acc[r][2 * jj]);
+          acc[r][2 * jj + 1] = MatrixOps<T>::k32(odd, p2[r], acc[r][2 * jj + 1]);
         }
       }
     }
@@ -502,13 +530,16 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
       page0 = page_of(nxt.b, first_tile(nxt));
       page1 = page_of(nxt.b, first_tile(nxt) + kUnit);
     }
-    m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int j = 0; j < kSlice; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < kM; ++r) {
+      m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kSlice; ++j) acc[r][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
     int tile = first_tile(cur);
     const bool any = tile < cur.t1;
     for (; tile + kUnit < cur.t1; tile += kUnit) {
-      f32x4 st[kSets];
+      f32x4 st[kM][kSets];
       const int page = page_of(cur.b, tile + 2 * kUnit);
       scores(st);
       publish(cur.t1, tile + kUnit, next);
@@ -518,7 +549,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
       next = page;
     }
     {
-      f32x4 st[kSets];
+      f32x4 st[kM][kSets];
       const bool next_any = more && first_tile(nxt) < nxt.t1;
       if (any) scores(st);
       if (next_any) {
@@ -532,37 +563,43 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes))
         next = page1;
       }
     }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-
-    // ---- the waves' sums together
-    const bool whole = cur.from == 0 && cur.to == cur.units;
-    const int64_t part = (((int64_t)hg * a.shares + share) * 2 + (cur.from == 0 ? 1 : 0)) * 16;
 #pragma unroll
-    for (int j0 = 0; j0 < kSlice; j0 += kJ) {
+    for (int r = 0; r < kM; ++r) {
+      l[r] += __shfl_xor(l[r], 16, 64);
+      l[r] += __shfl_xor(l[r], 32, 64);
+    }
+
+    // ---- the waves' sums together, sixteen rows and kJ channels of each slice at a time
+    const bool whole = cur.from == 0 && cur.to == cur.units;
+    const int64_t part = (((int64_t)hg * a.shares + share) * 2 + (cur.from == 0 ? 1 : 0)) * (16 * kM);
+#pragma unroll
+    for (int pass = 0; pass < kM * (kSlice / kJ); ++pass) {
+      constexpr int kSlices = kSlice / kJ;
+      const int mr = pass / kSlices, j0 = pass % kSlices * kJ;
+      if (16 * mr >= rows) break;
       lds_barrier();   // (what the last pass or stretch left there has been read)
-      if (c < rows) {
-        if (g == 0) sm_m[wave][c] = m, sm_l[wave][c] = l;
+      if (16 * mr + c < rows) {
+        if (g == 0) sm_m[wave][c] = m[mr], sm_l[wave][c] = l[mr];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < kJ; ++j) sm_acc[wave][c][(4 * g + i) * kJ + j] = acc[j0 + j][i];
+          for (int j = 0; j < kJ; ++j) sm_acc[wave][c][(4 * g + i) * kJ + j] = acc[mr][j0 + j][i];
       }
       lds_barrier();
-      const int row = threadIdx.x >> 4, r = threadIdx.x & 15;
+      const int in_pass = threadIdx.x >> 4, r = threadIdx.x & 15, row = 16 * mr + in_pass;
       if (row < rows) {
-        float mx = sm_m[0][row];
+        float mx = sm_m[0][in_pass];
 #pragma unroll
-        for (int w = 1; w < kPagedWaves; ++w) mx = fmaxf(mx, sm_m[w][row]);
+        for (int w = 1; w < kPagedWaves; ++w) mx = fmaxf(mx, sm_m[w][in_pass]);
         float sum = 0.f, at[kJ];
 #pragma unroll
         for (int j = 0; j < kJ; ++j) at[j] = 0.f;
 #pragma unroll
         for (int w = 0; w < kPagedWaves; ++w) {
-          const float by = mx == -INFINITY ? 1.f : fast_exp2(sm_m[w][row] - mx);
-          sum += sm_l[w][row] * by;
+          const float by = mx == -INFINITY ? 1.f : fast_exp2(sm_m[w][in_pass] - mx);
+          sum += sm_l[w][in_pass] * by;
 #pragma unroll
-          for (int j = 0; j < kJ; ++j) at[j] += sm_acc[w][row][r * kJ + j] * by;
+          for (int j = 0; j < kJ; ++j) at[j] += sm_acc[w][in_pass][r * kJ + j] * by;
         }
         write_sums<T, Tile, kJ>(a, whole, (int64_t)cur.b * a.n_q_heads + first_q + row, part + row, kD, r, j0, mx, sum,
                                 v_scale, at);
@@ -600,8 +637,9 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedAr
   const int s0 = begin / each, n = (end - 1) / each - s0 + 1;
   if (n == 1) return;
   const int h = hq / a.rep, rr = hq - h * a.rep;
-  const int64_t hg = (int64_t)h * a.groups + rr / 16;
-  auto row = [&](int i) { return ((hg * a.shares + s0 + i) * 2 + (i == 0 ? 1 : 0)) * 16 + rr % 16; };
+  const int64_t hg = (int64_t)h * a.groups + rr / a.group_rows;
+  const int in_group = rr % a.group_rows;
+  auto row = [&](int i) { return ((hg * a.shares + s0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group_rows + in_group; };
 
   // the parts' maxima and sums: each thread a few, then by the block
   constexpr int kOwn = kPagedMostShares / kPagedThreads;
@@ -664,12 +702,17 @@ int launch_paged_dim(const PagedArgs &a, hipStream_t s) {
   // Keys and values that are read once come by streaming where their rows are whole lines: 137 instead of 154 us for 834 MB
   // of e4m3 rows of 128, 88 instead of 99 for 128K tokens of bf16 ones, the same for fp32 ones of 256.  Rows that share
   // lines are read faster through the caches (bf16 ones of 96: 191 instead of 211 us for 1 GB, e4m3 ones of 64: 195, 220), and
-  // so are those that several groups of query heads read (64/2 heads: 216 instead of 278).
+  // so are those that several groups of query heads read (two of 16 of 64/2 heads of 128: 216 instead of 278).
   constexpr bool kWholeLines = kD * KV::kBytes % 128 == 0;
-  if (kWholeLines && a.groups == 1)
-    hipLaunchKernelGGL((paged_attention_kernel<T, KV, kD, kWholeLines>), dim3(blocks), dim3(kPagedThreads), 0, s, a);
-  else
-    hipLaunchKernelGGL((paged_attention_kernel<T, KV, kD, false>), dim3(blocks), dim3(kPagedThreads), 0, s, a);
+  const bool stream = kWholeLines && a.groups == 1;
+#define DA_PAGED(streaming, sixteens)                                                                              \
+  hipLaunchKernelGGL((paged_attention_kernel<T, KV, kD, streaming, sixteens>), dim3(blocks), dim3(kPagedThreads), 0, s, a)
+  constexpr int kMost = paged_sixteens(kD, T::kBytes, 32);
+  if (a.group_rows > 16 && stream) DA_PAGED(kWholeLines, kMost);
+  else if (a.group_rows > 16) DA_PAGED(false, kMost);
+  else if (stream) DA_PAGED(kWholeLines, 1);
+  else DA_PAGED(false, 1);
+#undef DA_PAGED
   if (a.shares > 1) {
     const bool by_border = a.shares - 1 < a.n_seqs;
     const unsigned joins = (unsigned)a.n_q_heads * (unsigned)(by_border ? a.shares - 1 : a.n_seqs);

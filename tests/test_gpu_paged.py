@@ -217,6 +217,15 @@ def test_attention_of_groups_of_any_size(types, heads):
     check_attention(args, scales)
 
 
+@pytest.mark.parametrize("heads", [(17, 1, 128), (64, 2, 96), (100, 2, 128), (33, 1, 256)], ids=str)
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
+def test_attention_of_large_groups_at_every_head_size(types, heads):
+    dtype, cache = types
+    Hq, H, D = heads
+    args, scales = attention_case(gen(Hq), [0, 31, 1100, 129, 400], Hq, H, D, dtype, cache)
+    check_attention(args, scales)
+
+
 @pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
 @pytest.mark.parametrize("lengths", [[20000], [3001, 1], [1, 9000, 2, 0, 5000], [0, 0, 12345, 0]], ids=str)
 def test_attention_split_over_long_sequences(types, lengths):
