@@ -5,10 +5,10 @@ namespace da {
 
 constexpr int kComputeUnits = 256;
 // A sequence is one workgroup's where the table holds no more than this many tokens of it: joining costs a launch and
-// sharing out a scan.  Up to 512 tokens it always pays (one sequence of 256 of 32/8 heads 6.5 instead of 9.0 us, of 512 9.3 and
-// 9.1, 64 of 512 22.7 and 27.2), up to 1024 where there are workgroups for every compute unit twice (64 sequences of 1024
-// 42.7 and 47.0, of unlike lengths 33.9 and 36.1, but 16 of them 21.5 and 18.1); beyond, unlike lengths leave most of the chip
-// waiting for the longest (64 of up to 4096 124 and 85).
+// sharing out a scan.  Up to 512 tokens it always pays (one sequence of 256 of 32/8 heads 6.5 instead of 9.0 us, of 512
+// 9.3 and 9.1, 64 of 512 22.7 and 27.2), up to 1024 where there are workgroups for every compute unit twice (64
+// sequences of 1024 42.7 and 47.0, of unlike lengths 33.9 and 36.1, but 16 of them 21.5 and 18.1); beyond, unlike lengths
+// leave most of the chip waiting for the longest (64 of up to 4096 124 and 85).
 constexpr int kPagedDirect = 512, kPagedDirectMany = 1024;
 
 constexpr int64_t kPagedMostTokens = (int64_t)1 << 30;   // of a sequence: tiles ahead are counted in 32 bits
@@ -107,7 +107,8 @@ extern "C" int da_paged_attention(const void *args, size_t args_bytes, void *str
   a.lengths = r.lengths, a.lengths64 = r.length_type;
   a.n_seqs = r.n_sequences, a.n_pages = r.n_pages, a.max_tokens = most;
   a.by_page = divisor_of(r.page_size);
-  a.n_q_heads = r.n_q_heads, a.n_kv_heads = r.n_kv_heads, a.rep = r.n_q_heads / r.n_kv_heads, a.groups = plan.groups, a.group_rows = plan.group_rows;
+  a.n_q_heads = r.n_q_heads, a.n_kv_heads = r.n_kv_heads, a.rep = r.n_q_heads / r.n_kv_heads;
+  a.groups = plan.groups, a.group_rows = plan.group_rows;
   a.shares = plan.shares;
   a.scale_log2 = r.scale * kLog2e;
   a.k_scale = r.k_scale, a.v_scale = r.v_scale;

@@ -11,10 +11,11 @@
 // the millionth position of the fastest pair.  Whole turns go away in 64 bits, then quarters of a turn, and sine and
 // cosine of the rest are Taylor polynomials on |t| <= pi/4 (their next terms are below 2^-26).
 //
-// Bound: HBM; a row is read once and written once, up to 16 bytes a lane.  A workgroup takes a few tokens: its threads
-// form their angles, about one pair each, into LDS, while the first rows are on their way.  Its waves then take blocks of
-// 64 items (a load and a store each) of a token's head rows laid end to end, kInFlight blocks at a time; which token,
-// tensor and block it is, is the same for the whole wave and left to the scalar unit.
+// Bound: HBM; a row is read once and written once, up to 16 bytes a lane (16384 tokens of 32/8 heads of 128 in bf16
+// 60 us = 5.6 TB/s).  A workgroup takes a few tokens: its threads form their angles, about one pair each, into LDS, while
+// the first rows are on their way.  Its waves then take blocks of 64 items (a load and a store each) of a token's
+// head rows laid end to end, kInFlight blocks at a time; which token, tensor and block it is, is the same for the whole
+// wave and left to the scalar unit.
 #include "paged_math.hpp"
 
 namespace da {
@@ -287,7 +288,8 @@ static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int n, const c
 
 // Bytes read and written from which rows come and go by streaming: the last-level cache holds 256 MiB and would
 // keep none of them until they are used.  16384 tokens of 32/8 heads of 128 in bf16 (320 MiB) 72 -> 62 us, prompts of
-// 30720 tokens into pages (720 MiB) 163 -> 153; 4900 tokens of fp16 heads (58 MiB) 14 -> 20, their rows still in the cache.
+// 30720 tokens into pages (720 MiB) 163 -> 153; 4900 tokens of fp16 heads (58 MiB) 14 -> 20, their rows still in
+// the cache.
 constexpr int64_t kStreamBytes = (int64_t)256 << 20;
 
 template <typename T, typename TC, bool kPaged>
