@@ -59,7 +59,7 @@ static int check_paged(const da_paged_attention_args &r) {
     return fail(DA_ENOTSUP, "%s: head_dim 64, 96, 128 or 256 (got %d)", what, r.head_dim);
   if (paged_room(r) > kPagedMostTokens || r.n_q_heads > 1 << 16 ||
       (int64_t)r.n_sequences * r.n_q_heads > 0x7fffffff ||
-      r.n_sequences * (paged_room(r) / 64 + 1) > 0x7fffffff)
+      r.n_sequences * (paged_room(r) / 64 + 1) > 0x7fff0000)   // (units, and shares behind them, in 32 bits)
     return fail(DA_ENOTSUP, "%s: too many tokens or heads", what);
   return DA_OK;
 }

@@ -95,16 +95,13 @@ struct PagedTile {
   }
 };
 
-// log2(e) is in the scores already, so weights are powers of two.  fp16 weights are taken 2^11 times
-// themselves and rescaled early, so that small ones keep their bits: they are 0 below 2^-36 of the largest.
+// log2(e) is in the scores already, so weights are powers of two, at most 2^kWeightBias<T>: 1, but for fp16 2^15, so that
+// small weights keep their bits (they are 0 below 2^-40 of the largest).  The running maximum is followed at once: a lag,
+// which would spare rescaling, gains nothing here (711 to 713 us either way) and large values would overflow.
 template <typename T>
-struct WeightRange {
-  static constexpr float kSlack = kRescaleSlack, kBias = 0.f;
-};
+constexpr float kWeightBias = 0.f;
 template <>
-struct WeightRange<F16> {
-  static constexpr float kSlack = 4.f, kBias = 11.f;
-};
+inline constexpr float kWeightBias<F16> = 15.f;
 
 // Two e4m3 as two elements of T, exactly: the low or high half of w.
 template <typename T, bool kHigh>
@@ -194,7 +191,7 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
   constexpr int kHeld = 4 * kSets;                       // tokens whose scores and values a lane holds
   constexpr int kJ = kSlice > 8 ? 8 : kSlice;            // channels of a slice that are joined at a time
   constexpr int kRow = 16 * kJ + 4;                      // floats; the pad spreads rows over banks
-  using Range = WeightRange<T>;
+  constexpr float kBias = kWeightBias<T>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
 
   __shared__ int64_t offsets[kPagedWaves][kTokens];
@@ -437,8 +434,8 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
         p[r][x] = live >> x & 1 ? st[r][x / 4][x % 4] * scale_log2 : -INFINITY;
         top = fmaxf(top, p[r][x]);
       }
-      if (__any(top > m[r] + (Range::kSlack + Range::kBias))) {   // rare
-        float mx = top - Range::kBias;
+      if (__any(top > m[r] + kBias)) {
+        float mx = top - kBias;
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(fmaxf(mx, __shfl_xor(mx, 32, 64)), m[r]);
         const float alpha = mx == -INFINITY ? 1.f : fast_exp2(m[r] - mx);

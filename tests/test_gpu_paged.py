@@ -328,6 +328,22 @@ def test_scores_of_any_size(dtype):
         assert not far, far
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_values_near_the_largest_of_their_type(dtype):
+    """Scores that rise a little from tile to tile, and large values under the largest weight: no sum is above it."""
+    n = 400
+    args, _ = attention_case(gen(25), [n], 1, 1, 64, dtype)
+    q, kp, vp, table, lengths = args
+    q.zero_(), kp.zero_()
+    q[0, 0, 0] = 1
+    large = {torch.bfloat16: 2.0 ** 127, torch.float16: 60000.0, torch.float32: 2.0 ** 127}[dtype]
+    for t in range(n):
+        kp[int(table[0, t // 16]), t % 16, 0, 0] = (t // 32) * 0.5
+    kp[int(table[0, (n - 1) // 16]), (n - 1) % 16, 0, 0] = 9.0          # (6.0 is the largest of the others)
+    vp[int(table[0, (n - 1) // 16]), (n - 1) % 16, 0] = large
+    check_attention(args, {}, scale=1.0)
+
+
 def test_fp16_weights_of_many_small_scores_are_not_lost():
     """One token far above 60000 others that together weigh as much."""
     n = 60001
