@@ -15,8 +15,8 @@ constexpr int64_t kPagedMostTokens = (int64_t)1 << 30;   // of a sequence: tiles
 
 struct PagedPlan {
   int32_t groups, group_rows, shares;
-  size_t prefix_bytes, ml_bytes, acc_bytes;
-  size_t bytes() const { return shares > 1 ? prefix_bytes + ml_bytes + acc_bytes : 0; }
+  size_t prefix_bytes, border_bytes, ml_bytes, acc_bytes;
+  size_t bytes() const { return shares > 1 ? prefix_bytes + border_bytes + ml_bytes + acc_bytes : 0; }
 };
 
 static int64_t paged_room(const da_paged_attention_args &r) { return (int64_t)r.pages_per_sequence * r.page_size; }
@@ -38,6 +38,7 @@ static PagedPlan paged_plan(const da_paged_attention_args &r) {
   p.shares = (int32_t)shares;
   const int64_t rows = head_groups * shares * 2 * p.group_rows;
   p.prefix_bytes = (size_t)ceil_div(((int64_t)r.n_sequences + 1) * 4, 16) * 16;
+  p.border_bytes = (size_t)shares * 16;
   p.ml_bytes = (size_t)rows * 2 * 4;
   p.acc_bytes = (size_t)rows * r.head_dim * 4;
   return p;
@@ -115,8 +116,9 @@ extern "C" int da_paged_attention(const void *args, size_t args_bytes, void *str
   a.out = (char *)r.out, a.lse = r.lse;
   if (plan.bytes()) {
     a.prefix = (int32_t *)r.workspace;
-    a.part_ml = (float *)((char *)r.workspace + plan.prefix_bytes);
-    a.part_acc = (float *)((char *)r.workspace + plan.prefix_bytes + plan.ml_bytes);
+    a.borders = (int4 *)((char *)r.workspace + plan.prefix_bytes);
+    a.part_ml = (float *)((char *)a.borders + plan.border_bytes);
+    a.part_acc = (float *)((char *)a.part_ml + plan.ml_bytes);
   }
   hipStream_t s = (hipStream_t)stream;
   if (r.page_dtype == DA_E4M3)

@@ -67,6 +67,8 @@ struct PagedArgs {
   float *lse;
   float *part_acc, *part_ml;                    // [head group][share][2][row]
   int32_t *prefix;                              // units before sequence b; [n_seqs]: all
+  int4 *borders;                                // [share]: the sequence that its border with the share ahead is the first
+                                                // inside of (or -1), its first and end unit, units of a share
 };
 
 // How the two products take keys and values of type KV under queries of type T.
@@ -251,10 +253,14 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
       __syncthreads();
       const int each = (total + a.shares - 1) / a.shares, begin = min(share * each, total);
       int at = upto - sum;
-      if (blockIdx.x == 0) {
+      if (blockIdx.x == 0) {   // what the join asks for
+        for (int i = threadIdx.x; i < a.shares; i += kPagedThreads) a.borders[i] = make_int4(-1, 0, 0, 0);
+        __syncthreads();
         for (int i = first, n = at; i < last; ++i) {
+          const int end = n + (sequence_length(a, i) + kUnit - 1) / kUnit;
           a.prefix[i] = n;
-          n += (sequence_length(a, i) + kUnit - 1) / kUnit;
+          if (end > n && (n / each + 1) * each < end) a.borders[n / each + 1] = make_int4(i, n, end, each);
+          n = end;
         }
         if (threadIdx.x == 0) a.prefix[a.n_seqs] = total;
       }
@@ -611,67 +617,62 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
 }
 
 // The sums of sequences that more than one share holds: a workgroup for each query head and sequence or, where
-// there are fewer, inner border of two shares (the first one inside a sequence finds it).
+// there are fewer, inner border of two shares.  Bound: its launch and three rounds to memory, one for the stretch of shares,
+// one for all that they left (which waits for no weights), one for the output: every wave forms the weights for itself.
 template <typename T, int kD>
 __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedArgs a, const bool by_border) {
-  constexpr int kLanes = kD / 4, kParts = kPagedThreads / kLanes;
+  constexpr int kLanes = kD / 4, kParts = kPagedThreads / kLanes, kAhead = 8;
   __shared__ __align__(16) float sums[kParts][kD];
-  __shared__ float red[kPagedWaves], ls[kPagedWaves], weight[kPagedMostShares];
+  __shared__ float weight[kPagedMostShares];
   const int hq = (int)(blockIdx.x % (unsigned)a.n_q_heads), at = (int)(blockIdx.x / (unsigned)a.n_q_heads);
-  const int total = a.prefix[a.n_seqs];
-  const int each = (total + a.shares - 1) / a.shares;
-  int b = at;
+  const int lane = threadIdx.x & 63;
+  int b = at, s0, n;
   if (by_border) {
-    const int border = (at + 1) * each;
-    if (border >= total) return;
-    int lo = 0, hi = a.n_seqs;   // prefix[lo] <= border < prefix[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (a.prefix[mid] <= border) lo = mid; else hi = mid;
-    }
-    b = lo;
-    if (a.prefix[b] == border || a.prefix[b] < border - each) return;
+    const int4 x = a.borders[at + 1];
+    if (x.x < 0) return;
+    b = x.x, s0 = at, n = (x.z - 1) / x.w - s0 + 1;
+  } else {
+    const int begin = a.prefix[b], end = a.prefix[b + 1], each = (a.prefix[a.n_seqs] + a.shares - 1) / a.shares;
+    if (begin == end) return;
+    s0 = begin / each, n = (end - 1) / each - s0 + 1;
+    if (n == 1) return;
   }
-  const int begin = a.prefix[b], end = a.prefix[b + 1];
-  if (begin == end) return;
-  const int s0 = begin / each, n = (end - 1) / each - s0 + 1;
-  if (n == 1) return;
   const int h = hq / a.rep, rr = hq - h * a.rep;
   const int64_t hg = (int64_t)h * a.groups + rr / a.group_rows;
   const int in_group = rr % a.group_rows;
   auto row = [&](int i) { return ((hg * a.shares + s0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group_rows + in_group; };
-
-  // the parts' maxima and sums: each thread a few, then by the block
-  constexpr int kOwn = kPagedMostShares / kPagedThreads;
-  float m[kOwn], mx = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int x = 0; x < kOwn; ++x) {
-    const int i = threadIdx.x + x * kPagedThreads;
-    m[x] = i < n ? a.part_ml[row(i) * 2] : -INFINITY;
-    mx = fmaxf(mx, m[x]);
-  }
-  mx = group_max<64>(mx);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-#pragma unroll
-  for (int x = 0; x < kOwn; ++x) {
-    const int i = threadIdx.x + x * kPagedThreads;
-    if (i >= n) break;
-    const float by = mx == -INFINITY ? 1.f : fast_exp2(m[x] - mx);
-    weight[i] = by;
-    l += a.part_ml[row(i) * 2 + 1] * by;
-  }
-  l = group_sum<64>(l);
-  if ((threadIdx.x & 63) == 0) ls[threadIdx.x >> 6] = l;
-  __syncthreads();
-  l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+  auto maximum_and_sum = [&](int i) {
+    return i < n ? *(const float2 *)(a.part_ml + row(i) * 2) : make_float2(-INFINITY, 0.f);
+  };
 
   const int part = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+  const float2 first = maximum_and_sum(lane);
+  f32x4 ahead[kAhead];
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) {
+    const int i = part + t * kParts;
+    ahead[t] = part < kParts && i < n ? *(const f32x4 *)(a.part_acc + row(i) * kD + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float mx = first.x;
+  for (int i = lane + 64; i < n; i += 64) mx = fmaxf(mx, maximum_and_sum(i).x);
+  mx = group_max<64>(mx);
+  float l = 0.f;
+  for (int i = lane; i < n; i += 64) {
+    const float2 x = i == lane ? first : maximum_and_sum(i);
+    const float by = mx == -INFINITY ? 1.f : fast_exp2(x.x - mx);
+    weight[i] = by;   // (the same from every wave)
+    l += x.y * by;
+  }
+  l = group_sum<64>(l);
+  __builtin_amdgcn_wave_barrier();
+
   if (part < kParts) {
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int i = part; i < n; i += kParts) sum += *(const f32x4 *)(a.part_acc + row(i) * kD + d) * weight[i];
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t)
+      if (part + t * kParts < n) sum += ahead[t] * weight[part + t * kParts];
+    for (int i = part + kAhead * kParts; i < n; i += kParts)
+      sum += *(const f32x4 *)(a.part_acc + row(i) * kD + d) * weight[i];
     *(f32x4 *)&sums[part][d] = sum;
   }
   __syncthreads();
