@@ -58,10 +58,12 @@ static int check_paged(const da_paged_attention_args &r) {
     DA_REQUIRE(t == DA_I32 || t == DA_I64, "%s: unknown integer type %d", what, t);
   if (r.head_dim != 64 && r.head_dim != 96 && r.head_dim != 128 && r.head_dim != 256)
     return fail(DA_ENOTSUP, "%s: head_dim 64, 96, 128 or 256 (got %d)", what, r.head_dim);
-  if (paged_room(r) > kPagedMostTokens || r.n_q_heads > 1 << 16 ||
-      (int64_t)r.n_sequences * r.n_q_heads > 0x7fffffff ||
-      r.n_sequences * (paged_room(r) / 64 + 1) > 0x7fff0000)   // (units, and shares behind them, in 32 bits)
-    return fail(DA_ENOTSUP, "%s: too many tokens or heads", what);
+  // (a launch counts 2^32 threads, 256 for a sequence and head; units of tokens, and shares behind them, are counted in
+  // 32 bits)
+  if (paged_room(r) > kPagedMostTokens || r.n_q_heads > 4096 || (int64_t)r.n_sequences * r.n_q_heads > 0xffffff ||
+      r.n_sequences * (paged_room(r) / 64 + 1) > 0x7fff0000)
+    return fail(DA_ENOTSUP, "%s: %d sequences of up to %lld tokens, %d heads, are too many", what, r.n_sequences,
+                (long long)paged_room(r), r.n_q_heads);
   return DA_OK;
 }
 

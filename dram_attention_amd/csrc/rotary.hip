@@ -276,11 +276,15 @@ static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int n, const c
   if (tokens > 0x7fffff00 / batch)   // (counted in 32 bits, a workgroup's tokens ahead)
     return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens are too many", what, (long long)batch, (long long)tokens);
   a.tokens = (int32_t)(batch * tokens);
-  // as many tokens as there are angles for every thread, while enough workgroups are left
+  // as many tokens as there are angles for every thread, while enough workgroups are left; more only where a launch,
+  // which counts 2^32 threads, would not hold them
+  const int64_t most = 0xffffff;
   a.group = 1;
-  while (a.group * 2 * (pairs > 1 ? pairs : 1) <= kTurnThreads && a.group * 2 <= 64 &&
-         a.tokens / (a.group * 2) >= kTurnGrid)
+  while (a.group < 64 && a.group * 2 * pairs <= kMaxTurns &&
+         ((a.group * 2 * pairs <= kTurnThreads && a.tokens / (a.group * 2) >= kTurnGrid) || a.tokens / a.group >= most))
     a.group *= 2;
+  if (ceil_div(a.tokens, a.group) > most)
+    return fail(DA_ENOTSUP, "%s: %lld sequences of %lld tokens are too many", what, (long long)batch, (long long)tokens);
   a.by_tokens = divisor_of((int32_t)tokens), a.by_blocks = divisor_of((int32_t)blocks);
   a.by_pairs = divisor_of(pairs > 1 ? pairs : 1);
   return DA_OK;

@@ -245,6 +245,73 @@ def test_attention_of_many_ragged_sequences():
     check_attention(args, scales)
 
 
+@pytest.mark.parametrize("dtype, heads, n", [(torch.float16, (1, 1, 64), 131072), (torch.bfloat16, (3, 1, 128), 131072),
+                                             (torch.bfloat16, (1, 1, 64), 200001)])
+def test_attention_of_one_sequence_in_as_many_shares_as_there_are(dtype, heads, n):
+    args, _ = attention_case(gen(26), [n], *heads, dtype, page=64)
+    check_attention(args, {})
+
+
+@pytest.mark.parametrize("width", [1, 64])
+def test_attention_of_more_sequences_than_16_bits_count(width):
+    """70000 sequences of 0 to 3 tokens, a workgroup each or in shares."""
+    g = gen(27)
+    B, n_pages = 70000, 500
+    kp, vp = P.pool(n_pages, 16, 1, 64, torch.float32, DEV, g)
+    table = torch.zeros(B, width, dtype=torch.int32)
+    table[:, 0] = torch.randint(0, n_pages, (B,), generator=g)
+    table, lengths = table.to(DEV), torch.randint(0, 4, (B,), generator=g).to(DEV)
+    q = randn(g, B, 1, 64, dtype=torch.float32)
+    got = paged_decode_attention(q, kp, vp, table, lengths)
+    k, v = (x[table[:, 0].long(), :3, 0].double() for x in (kp, vp))
+    scores = torch.einsum("bd,btd->bt", q[:, 0].double(), k) / 8
+    weights = torch.where(torch.arange(3, device=DEV) < lengths[:, None], (scores - scores.amax(1, keepdim=True)).exp(), 0.0)
+    want = torch.einsum("bt,btd->bd", weights / weights.sum(1, keepdim=True).clamp(min=1e-300), v)
+    size = v.abs().amax(1)
+    # (scores of up to 64 * 5 * 5 / 8 in fp32: off by (64 + 8) * 2^-24 of their products' sizes)
+    reach = torch.einsum("bd,btd->bt", q[:, 0].double().abs(), k.abs()).amax(1, keepdim=True) / 8
+    far = P.outside(got[:, 0], want.cpu(), (2.02 * (72 * 2.0 ** -24 * reach + 20 * 2.0 ** -24) * size).cpu() + 2.0 ** -24 * want.abs().cpu())
+    assert not far, far
+
+
+def test_operands_that_do_not_lie_in_a_row():
+    """Lengths, positions and sequences with gaps; one layer of a pool of several; page tables wider than they are used."""
+    g = gen(28)
+    args, _ = attention_case(g, [100, 1000, 7], 4, 2, 64, torch.bfloat16)
+    q, kp, vp, table, lengths = args
+    want = paged_decode_attention(*args)
+    spread = torch.zeros(6, dtype=torch.int64, device=DEV)
+    spread[::2] = lengths
+    layers = torch.full((3, *kp.shape), float("nan"), dtype=kp.dtype, device=DEV), torch.full((3, *kp.shape), float("nan"), dtype=kp.dtype, device=DEV)
+    layers[0][1], layers[1][1] = kp, vp
+    wide = torch.full((3, 2 * table.shape[1]), -1, dtype=torch.int64, device=DEV)
+    wide[:, : table.shape[1]] = table
+    assert torch.equal(paged_decode_attention(q, layers[0][1], layers[1][1], wide[:, : table.shape[1]], spread[::2]), want)
+    k, v = (randn(g, 3, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    at = torch.tensor([3, 0, 40, 0, 5, 0], device=DEV)[::2]
+    of = torch.tensor([2, 9, 0, 9, 1, 9], dtype=torch.int32, device=DEV)[::2]
+    append_kv_pages_(k, v, layers[0][1], layers[1][1], wide, at, sequences=of)
+    for t, (b, p) in enumerate(zip(of.tolist(), at.tolist())):
+        number = int(table[b, p // 16])
+        assert torch.equal(layers[0][1][number, p % 16], k[t]) and torch.equal(layers[1][1][number, p % 16], v[t])
+    assert layers[0][0].isnan().all() and layers[1][2].isnan().all()
+
+
+def test_eight_bit_pages_with_one_scale_or_none():
+    args, scales = attention_case(gen(29), [50, 700], 4, 2, 64, torch.bfloat16, E4M3)
+    q, kp, vp, table, lengths = args
+    ones = torch.ones(2, device=DEV)
+    for k_scale, v_scale in ((None, None), (scales["k_scale"], None), (None, scales["v_scale"])):
+        want = paged_decode_attention(*args, k_scale=ones if k_scale is None else k_scale,
+                                      v_scale=ones if v_scale is None else v_scale)
+        assert torch.equal(paged_decode_attention(*args, k_scale=k_scale, v_scale=v_scale), want)
+    k, v = (randn(gen(30), 2, 2, 64, dtype=torch.bfloat16) for _ in range(2))
+    append_kv_pages_(k, v, kp, vp, table, lengths - 1, v_scale=scales["v_scale"])
+    at = table[torch.arange(2), (lengths.cpu() - 1).long() // 16].long(), (lengths.long() - 1) % 16
+    assert torch.equal(bits(kp[at]), bits(k.to(E4M3)))
+    assert torch.equal(bits(vp[at]), bits((v.float() / scales["v_scale"][:, None]).to(E4M3)))
+
+
 def test_attention_of_empty_batches_tables_and_pools():
     args, _ = attention_case(gen(12), [5, 700], 4, 2, 64, torch.bfloat16)
     q, kp, vp, table, lengths = args

@@ -236,6 +236,8 @@ def test_c_entry_points_check_before_any_launch(lib):
     for bad, code in (({}, -1), ({"dtype": 3}, -1), ({"rotary_dim": 63}, -1), ({"rotary_dim": 66}, -1), ({"layout": 2}, -1),
                       ({"tokens": -1}, -1), ({"position_type": 5}, -1), ({"head_dim": 1024, "rotary_dim": 1024, "freqs": 16}, -2),
                       ({"tokens": 1 << 40, "q": 16, "k": 16, "q_out": 16, "k_out": 16, "freqs": 16, "positions": 16}, -2),
+                      ({"tokens": (1 << 31) - 300, "head_dim": 512, "rotary_dim": 512, "q": 16, "k": 16, "q_out": 16, "k_out": 16,
+                        "freqs": 16, "positions": 16}, -2),
                       ({"tokens": 0, "freqs": 16}, 0)):
         assert call(lib, "da_rotate", RotateArgs(**{**rot, **bad})) == code, bad
     app = dict(n_pages=4, page_size=16, n_sequences=2, pages_per_sequence=3, n_kv_heads=2, head_dim=64, dtype=2,
@@ -249,6 +251,7 @@ def test_c_entry_points_check_before_any_launch(lib):
     for bad, code in (({"q": None}, -1), ({"head_dim": 80}, -2), ({"n_q_heads": 3}, -1), ({"page_dtype": 0}, -1),
                       ({"dtype": 0, "page_dtype": 3}, -2), ({"v_scale": 16}, -1), ({"q": 8}, -1), ({}, -1),
                       ({"workspace": 16, "workspace_bytes": 64}, -1), ({"page_size": 1 << 28}, -2), ({"length_type": 7}, -1),
+                      ({"n_q_heads": 8192}, -2), ({"n_sequences": 1 << 23}, -2),
                       ({"q_strides": (ctypes.c_int64 * 2)(4, 64)}, -1), ({"n_sequences": 0}, 0)):
         assert call(lib, "da_paged_attention", AttentionArgs(**{**att, **bad})) == code, bad
     need = lib.da_paged_attention_workspace_bytes(bytes(AttentionArgs(**att)), ctypes.sizeof(AttentionArgs))
