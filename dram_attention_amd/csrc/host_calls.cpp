@@ -546,6 +546,7 @@ Turn read_turn(Args &in, int64_t head_dim) {
     TORCH_CHECK_VALUE(2 * t.freqs->numel() <= head_dim, t.freqs->numel(), " frequencies turn ", 2 * t.freqs->numel(),
                       " channels, but heads have ", head_dim);
     TORCH_CHECK_VALUE(t.freqs->numel() <= 256, "up to 256 frequencies (got ", t.freqs->numel(), ")");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !t.freqs->requires_grad(), "frequencies have no gradient");
   }
   return t;
 }

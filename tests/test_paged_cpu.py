@@ -71,6 +71,7 @@ def rotate_operands(**other):
     ({"freqs": torch.zeros(33, dtype=torch.float64)}, ValueError, "channels"),
     ({"freqs": torch.zeros(64, dtype=torch.float64)[::2]}, ValueError, "contiguous"),
     ({"freqs": None}, TypeError, "freqs"),
+    ({"freqs": torch.zeros(32, dtype=torch.float64, requires_grad=True)}, RuntimeError, "no gradient"),
     ({"layout": "both"}, ValueError, "layout"),
 ])
 def test_rotate_refuses(other, kind, match):
