@@ -512,8 +512,13 @@ void changed(const at::Tensor &t) {
 }
 int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 bool dense_rows(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
-// Rows as the kernels read them: the last axis dense, and where `vectors` 16-byte aligned.
+// Rows as the kernels read them: the last axis dense, and where `vectors` 16-byte aligned.  (A gradient may be a lazy
+// view of what its memory holds.)
 at::Tensor rows_of(const at::Tensor &t, bool vectors) {
+  if (t.is_neg() || t._is_zerotensor()) {
+    const Released others;
+    return t.is_neg() ? t.resolve_neg().contiguous() : at::zeros(t.sizes(), t.options().requires_grad(false));
+  }
   bool fits = dense_rows(t);
   if (vectors) {
     fits = fits && aligned(t);

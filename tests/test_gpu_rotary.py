@@ -142,6 +142,19 @@ def test_gradients_of_broadcast_rows_and_gradients_add_up():
     assert not far, far
 
 
+def test_gradients_that_are_lazy_views():
+    """What autograd hands over may be the negative, or nothing, of what its memory holds."""
+    g = gen(9)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(5, device=DEV)
+    q = randn(g, 5, 2, 64, dtype=torch.float32).requires_grad_()
+    y, _ = rotate(q, None, positions, freqs)
+    negative = torch.randn(5, 2, 64, dtype=torch.complex64, generator=g).to(DEV).conj().imag
+    assert negative.is_neg()
+    dq, = torch.autograd.grad(y, (q,), negative)
+    check(dq, negative.resolve_neg().contiguous(), -positions, freqs, "interleaved")
+
+
 def test_the_gradient_has_a_gradient():
     g = gen(5)
     q = randn(g, 5, 2, 64, dtype=torch.float32).requires_grad_()
