@@ -18,6 +18,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -536,6 +537,21 @@ at::Tensor in_line(const at::Tensor &t) {   // a one-dimensional operand
 
 void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
+// A leaf that an eager graph holds has the place where its gradient arrives on that graph's stream: a backward pass
+// that is captured would lead there, out of the capture, and take the process down.  Refused while it is harmless.
+void no_eager_graph_of(const at::Tensor &t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto arrival = torch::autograd::impl::try_get_grad_accumulator(t);
+  // (By number: torch's graphs call the device cuda, c10::hip calls it hip.)
+  if (!arrival || !arrival->stream() || arrival->stream()->id() == c10::hip::getCurrentHIPStream(t.device().index()).id())
+    return;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  const hipError_t rc = hipStreamIsCapturing((hipStream_t)stream_of(t), &status);
+  TORCH_CHECK(rc == hipSuccess && status == hipStreamCaptureStatusNone,
+              "a leaf of this captured call is still held by an eager graph: drop that graph's results first, or capture "
+              "under torch.no_grad()");
+}
+
 // How a call turns channels: frequencies (or none), layout, factor.
 struct Turn {
   const at::Tensor *freqs;
@@ -693,6 +709,8 @@ PyObject *rotate(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
     }
     y = turn_rows(xq, xk ? *xk : at::Tensor(), positions, turn, false, true);
   } else if (at::GradMode::is_enabled() && (xq.requires_grad() || (xk && xk->requires_grad()))) {
+    no_eager_graph_of(xq);
+    if (xk) no_eager_graph_of(*xk);
     auto out = Turned::apply(xq, xk ? std::optional<at::Tensor>(*xk) : std::nullopt, positions, *turn.freqs, turn.half,
                              turn.factor, false);
     y = {out[0], xk ? out[1] : at::Tensor()};

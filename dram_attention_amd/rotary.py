@@ -99,7 +99,7 @@ def rotate(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, f
     positions int32 or int64, one per token: (tokens,), or (batch, tokens).  ``layout``: which channels turn together,
     2i and 2i + 1 ("interleaved", as llama.py's checkpoints have them) or i and i + len(freqs) ("half").  ``freqs`` and
     ``factor`` are :func:`rotary_frequencies`'s.  bf16, fp16 or fp32 with any strides; products in fp32, rounded once.
-    (A captured backward pass needs leaves that no eager graph still holds, as torch's own operators do.)
+    A call with gradients that is captured into a graph refuses leaves that an eager graph still holds.
     """
     if forward_ad._current_level >= 0:
         raise RuntimeError("rotate has no forward-mode derivative")

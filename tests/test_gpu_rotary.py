@@ -236,6 +236,34 @@ def test_what_is_turned_in_place_is_noticed_by_a_graph_that_needs_it():
         y.backward()
 
 
+def test_a_captured_call_refuses_leaves_that_an_eager_graph_holds():
+    """(Refused ahead of the first launch; the same leaves are taken once the eager graph is gone.)"""
+    g = gen(10)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(6, device=DEV)
+    x, gr = randn(g, 6, 2, 64, dtype=torch.bfloat16).requires_grad_(), randn(g, 6, 2, 64, dtype=torch.bfloat16)
+    eager, _ = rotate(x, None, positions, freqs)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="held by an eager graph"):
+            rotate(x, None, positions, freqs)
+        with torch.no_grad():
+            rotate(x, None, positions, freqs)       # (without gradients nothing leads there)
+    want = eager.detach().clone()
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, _ = rotate(x, None, positions, freqs)
+        again, _ = rotate(x, None, positions, freqs)
+        dx, = torch.autograd.grad((y, again), (x,), (gr, gr))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(again, want)
+        back = rotate(gr, None, -positions, freqs)[0]
+        assert torch.equal(dx, back + back)
+
+
 def test_many_waves():
     """More waves than a grid's first dimension has threads in one workgroup, heads in several windows."""
     T, H, D = 20011, 9, 64
