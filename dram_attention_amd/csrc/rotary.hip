@@ -292,7 +292,7 @@ static int shape_rows(TurnArgs &a, int64_t batch, int64_t tokens, int n, const c
 
 // Bytes read and written from which rows come and go by streaming: the last-level cache holds 256 MiB and would
 // keep none of them until they are used.  16384 tokens of 32/8 heads of 128 in bf16 (320 MiB) 72 -> 62 us, prompts of
-// 30720 tokens into pages (720 MiB) 163 -> 153; 4900 tokens of fp16 heads (58 MiB) 14 -> 20, their rows still in
+// 30 thousand tokens into pages (720 MiB) 163 -> 153; 4900 tokens of fp16 heads (58 MiB) 14 -> 20, their rows still in
 // the cache.
 constexpr int64_t kStreamBytes = (int64_t)256 << 20;
 
