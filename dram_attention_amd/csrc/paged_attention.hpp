@@ -17,9 +17,8 @@
 //                                     B operand as it stands, if the product's k index counts tokens in that order
 // V^T is the A operand: lane (g, c) holds its 8 tokens of one channel.  A lane loads the slice of D/16 channels that is
 // its own of each of its 8 tokens (whole rows per instruction) and pairs the tokens' halves up by byte permutes, 4 a
-// channel, so V needs no LDS.  Weights go in as sums of two 16-bit numbers
-// (split_weights), so that they keep 16 bits: the matrix cores have the room, and the result's error is that of its own
-// rounding.  fp32: tiles of 16 tokens, the same layouts with k = 4, nothing is rounded.
+// channel, so V needs no LDS.  Weights go in as sums of 16-bit numbers (split_weights), three in bf16, so that they keep
+// their bits: the matrix cores have the room.  fp32: tiles of 16 tokens, the same layouts with k = 4, nothing is rounded.
 // e4m3 keys and values become 16-bit ones (exactly) in registers; their heads' scales go into the scores and the output.
 //
 // The K registers are loaded anew as soon as the scores are formed, the V registers as soon as they are consumed, page
@@ -114,20 +113,30 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, kHigh));
 }
 
-// Two weights as the sums of two numbers of T each (dwords).  The first number is below the weight, so that both are
-// positive: an infinite value times them is infinite, where a rest of 0 or less would make NaN of it.  What is left out is
-// at most 2^-15 of a weight (bf16: the rest is at most 2^-7 of it) or 1.5 * 2^-21 (fp16: 1.5 * 2^-10).
+// Numbers of T that a weight is the sum of: three bf16 ones hold the 24 bits of fp32 (two left out up to 2^-15 of a weight;
+// the third costs 128K tokens of heads of 128 and 16 sequences to 128K nothing, heads of 64 1-2 %, 8-bit rows 1-3 %, 32
+// query rows a wave 6 %), two fp16 ones all but 1.5 * 2^-21 of a weight, as the second is at most 1.5 * 2^-10 of it.
 template <typename T>
-__device__ __forceinline__ void split_weights(float lo, float hi, uint32_t &first, uint32_t &rest) {
+constexpr int kWeightParts = __is_same(T, BF16) ? 3 : 2;
+
+// Two weights as such sums, dword i of part i.  Every part but the last is below what is left of the weight, so that all
+// are positive: an infinite value times them is infinite, where a rest of 0 or less would make NaN of it.
+__device__ __forceinline__ uint32_t take_bf16_below(float &lo, float &hi) {
+  const uint32_t a = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, lo), 1u);
+  const uint32_t b = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, hi), 1u);
+  lo -= as_f32(a & 0xffff0000u), hi -= as_f32(b & 0xffff0000u);
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+template <typename T>
+__device__ __forceinline__ void split_weights(float lo, float hi, uint32_t (&part)[kWeightParts<T>]) {
   if constexpr (__is_same(T, BF16)) {
-    const uint32_t a = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, lo), 1u);
-    const uint32_t b = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, hi), 1u);
-    first = __builtin_amdgcn_perm(b, a, 0x07060302u);
-    rest = pack_bf16(lo - as_f32(a & 0xffff0000u), hi - as_f32(b & 0xffff0000u));
+    part[0] = take_bf16_below(lo, hi);
+    part[1] = take_bf16_below(lo, hi);
+    part[2] = pack_bf16(lo, hi);
   } else {
     constexpr float kBelow = 1.f - 1.f / 2048;
-    first = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo * kBelow, hi * kBelow));
-    rest = pack_f16(lo - f16_lo(first), hi - f16_hi(first));
+    part[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo * kBelow, hi * kBelow));
+    part[1] = pack_f16(lo - f16_lo(part[0]), hi - f16_hi(part[0]));
   }
 }
 
@@ -473,14 +482,16 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
           for (int r = 0; r < kM; ++r)
             acc[r][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(as_f32(vv[x][j]), p[r][x], acc[r][j], 0, 0, 0);
     } else {
-      u32x4 p1[kM], p2[kM];
+      constexpr int kParts = kWeightParts<T>;
+      u32x4 parts[kM][kParts];
 #pragma unroll
       for (int r = 0; r < kM; ++r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t first, rest;
-          split_weights<T>(p[r][2 * i], p[r][2 * i + 1], first, rest);
-          p1[r][i] = first, p2[r][i] = rest;
+          uint32_t part[kParts];
+          split_weights<T>(p[r][2 * i], p[r][2 * i + 1], part);
+#pragma unroll
+          for (int n = 0; n < kParts; ++n) parts[r][n][i] = part[n];
         }
 #pragma unroll
       for (int jj = 0; jj < kSlice / 2; ++jj) {   // a dword: channels 2jj, 2jj + 1 of each token
@@ -499,12 +510,12 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
           odd[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
         }
 #pragma unroll
-        for (int r = 0; r < kM; ++r) {
-          acc[r][2 * jj] = MatrixOps<T>::k32(even, p1[r], acc[r][2 * jj]);
-          acc[r][2 * jj + 1] = MatrixOps<T>::k32(odd, p1[r], acc[r][2 * jj + 1]);
-          acc[r][2 * jj] = MatrixOps<T>::k32(even, p2[r], acc[r][2 * jj]);
-          acc[r][2 * jj + 1] = MatrixOps<T>::k32(odd, p2[r], acc[r][2 * jj + 1]);
-        }
+        for (int n = 0; n < kParts; ++n)
+#pragma unroll
+          for (int r = 0; r < kM; ++r) {
+            acc[r][2 * jj] = MatrixOps<T>::k32(even, parts[r][n], acc[r][2 * jj]);
+            acc[r][2 * jj + 1] = MatrixOps<T>::k32(odd, parts[r][n], acc[r][2 * jj + 1]);
+          }
       }
     }
   };

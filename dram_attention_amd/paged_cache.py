@@ -61,7 +61,7 @@ def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     include the token itself where its key was stored before.  ``scale``: head_dim ** -0.5 by default.  Returns a tensor
     like xq (``out`` if given); fills ``lse`` (sequences, heads) fp32, the natural logarithm of the softmax denominator.
     A sequence of no tokens gets zeros (lse -inf), and tokens on pages that are none of the pool's do not count.
-    16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, by weights that are kept to 2^-15 (bf16)
-    or 2^-20 (fp16) of themselves; fp32 ones are multiplied in fp32.  The same shapes and lengths give the same bits.
+    16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, by weights of 24 bits (bf16) or ones that
+    are kept to 2^-20 of themselves (fp16); fp32 ones are multiplied in fp32.  The same shapes and lengths give the same bits.
     """
     return _lib.host().paged_attention(xq, k_pages, v_pages, page_table, lengths, scale, k_scale, v_scale, out, lse)

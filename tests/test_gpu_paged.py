@@ -639,3 +639,29 @@ def test_decoding_a_batch_against_attention_over_its_history(types):
             far = P.outside(out[b:b + 1], o, bound)
             assert not far, (s, b, far)
         at.add_(1)
+
+
+@pytest.mark.parametrize("n", [15, 30, 60])
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
+def test_weights_keep_their_bits(types, n):
+    """One token against n that weigh 1/n each: what is left of the sum shows what a weight has lost."""
+    dtype, cache = types
+    args, scales = attention_case(gen(31), [n + 1], 2, 1, 64, dtype, cache)
+    q, kp, vp, table, _ = args
+    q.zero_()
+    q[:, :, 0] = 1
+    key, value = torch.zeros(n + 1, 64), torch.full((n + 1, 64), -1.0)
+    key[1:, 0], value[0] = 1, 1
+    for t in range(n + 1):
+        at = int(table[0, t // 16])
+        kp[at, t % 16, 0], vp[at, t % 16, 0] = key[t].to(kp.dtype).to(DEV), value[t].to(vp.dtype).to(DEV)
+    ones = {name: torch.ones_like(x) for name, x in scales.items()}
+    scale = float(torch.tensor(-math.log(n)))
+    out, _, size, reach = P.attention(*args, scale)
+    got = paged_decode_attention(*args, scale=scale, **ones)
+    # a score is one product times the scale times log2 e: four half steps of it, the exponential eight of the weight;
+    # n + 1 weights and values are added up in fp32; fp16 weights are two numbers, off by 1.5 * 2^-21.  (The quotient's
+    # own errors are those of a number that is nearly nothing.)
+    relative = 2.0 ** -24 * (4 * reach + 8 + n + 8) + (1.5 * 2.0 ** -21 if dtype == torch.float16 else 0.0)
+    far = P.outside(got, out, (relative[..., None] * (size + 2 * out.abs())) + P.HALF_STEP[dtype] * out.abs() + P.SMALLEST[dtype])
+    assert not far, far
