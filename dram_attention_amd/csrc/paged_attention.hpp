@@ -97,7 +97,7 @@ struct PagedTile {
 };
 
 // log2(e) is in the scores already, so weights are powers of two, at most 2^kWeightBias<T>: 1, but for fp16 2^15, so that
-// small weights keep their bits (they are 0 below 2^-40 of the largest).  The running maximum is followed at once: a lag,
+// small weights keep their bits (those below 2^-40 of the largest are 0).  The running maximum is followed at once: a lag,
 // which would spare rescaling, gains nothing here (711 to 713 us either way) and large values would overflow.
 template <typename T>
 constexpr float kWeightBias = 0.f;
@@ -115,12 +115,14 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t w) {
 
 // Numbers of T that a weight is the sum of: three bf16 ones hold the 24 bits of fp32 (two left out up to 2^-15 of a weight;
 // the third costs 128K tokens of heads of 128 and 16 sequences to 128K nothing, heads of 64 1-2 %, 8-bit rows 1-3 %, 32
-// query rows a wave 6 %), two fp16 ones all but 1.5 * 2^-21 of a weight, as the second is at most 1.5 * 2^-10 of it.
+// query rows a wave 6 %), two fp16 ones all but 1.5 * 2^-21 of a weight, as the second is at most 1.5 * 2^-10 of it,
+// or 2^-40 of the largest weight, half of fp16's least step, whichever is more.
 template <typename T>
 constexpr int kWeightParts = __is_same(T, BF16) ? 3 : 2;
 
 // Two weights as such sums, dword i of part i.  Every part but the last is below what is left of the weight, so that all
-// are positive: an infinite value times them is infinite, where a rest of 0 or less would make NaN of it.
+// are positive: an infinite value times them is infinite, where a rest of 0 or less would make NaN of it.  (So it is
+// down to 2^-29 of the largest weight in fp16, 2^-100 in bf16; smaller ones may have parts that are 0.)
 __device__ __forceinline__ uint32_t take_bf16_below(float &lo, float &hi) {
   const uint32_t a = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, lo), 1u);
   const uint32_t b = __builtin_elementwise_sub_sat(__builtin_bit_cast(uint32_t, hi), 1u);

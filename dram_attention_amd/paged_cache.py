@@ -62,6 +62,8 @@ def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     like xq (``out`` if given); fills ``lse`` (sequences, heads) fp32, the natural logarithm of the softmax denominator.
     A sequence of no tokens gets zeros (lse -inf), and tokens on pages that are none of the pool's do not count.
     16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, by weights of 24 bits (bf16) or ones that
-    are kept to 2^-20 of themselves (fp16); fp32 ones are multiplied in fp32.  The same shapes and lengths give the same bits.
+    are kept to 2^-20 of themselves or 2^-40 of the sequence's largest, whichever is more (fp16: an infinite value under a
+    weight below 2^-29 of the largest may give NaN); fp32 ones are multiplied in fp32.  The same shapes and lengths give the
+    same bits.
     """
     return _lib.host().paged_attention(xq, k_pages, v_pages, page_table, lengths, scale, k_scale, v_scale, out, lse)

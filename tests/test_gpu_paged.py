@@ -665,3 +665,45 @@ def test_weights_keep_their_bits(types, n):
     relative = 2.0 ** -24 * (4 * reach + 8 + n + 8) + (1.5 * 2.0 ** -21 if dtype == torch.float16 else 0.0)
     far = P.outside(got, out, (relative[..., None] * (size + 2 * out.abs())) + P.HALF_STEP[dtype] * out.abs() + P.SMALLEST[dtype])
     assert not far, far
+
+
+@pytest.mark.parametrize("dtype, below", [(torch.float16, 28), (torch.bfloat16, 28), (torch.bfloat16, 90), (torch.float32, 90)])
+@pytest.mark.parametrize("n", [200, 3000])
+def test_infinite_values_under_small_weights(dtype, below, n):
+    """An infinite value is one whatever its token weighs, as far as its weight has all its parts."""
+    args, _ = attention_case(gen(32), [n, n], 4, 2, 64, dtype)
+    q, kp, vp, table, _ = args
+    q.zero_()
+    q[:, :, 0] = 1
+    kp[..., 0] = 0
+    scale = below * math.log(2.0)
+    for t in range(n):      # (the largest weight is at the end of sequence 0 and at the beginning of sequence 1)
+        for b, top in ((0, n - 1), (1, 0)):
+            kp[int(table[b, t // 16]), t % 16, :, 0] = 1.0 if t == top else -0.01 * (t % 2)
+    clean = check_attention(args, {}, scale=scale)
+    last = (n - 1) // 32 * 32
+    # (beside the largest weight in its wave's tile of 32, in that wave's tile before or behind, in other waves')
+    for b, t in ((0, last + 1), (0, last - 126), (0, 3), (1, 1), (1, 130), (1, n - 2)):
+        vp[int(table[b, t // 16]), t % 16, 0, 5] = float("inf")
+        vp[int(table[b, t // 16]), t % 16, 1, 9] = -float("inf")
+    got = paged_decode_attention(*args, scale=scale)
+    assert (got[:, :2, 5] == float("inf")).all() and (got[:, 2:, 9] == -float("inf")).all()
+    got[:, :2, 5], got[:, 2:, 9] = clean[:, :2, 5], clean[:, 2:, 9]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("types", [(torch.bfloat16, E4M3), (torch.float16, E4M3), (torch.float16, None)],
+                         ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
+def test_missing_values_stay_with_their_sequence_and_head(types):
+    dtype, cache = types
+    args, scales = attention_case(gen(33), [200, 200, 700, 700], 4, 2, 64, dtype, cache)
+    q, kp, vp, table, _ = args
+    clean = paged_decode_attention(*args, **scales)
+    nan = torch.tensor(float("nan")).to(kp.dtype).to(DEV)
+    whole = torch.uint8 if cache else dtype
+    vp.view(whole)[int(table[0, 3]), 5, 1, 7] = nan.view(whole)
+    kp.view(whole)[int(table[3, 40]), 2, 0, 9] = nan.view(whole)
+    got = paged_decode_attention(*args, **scales)
+    assert got[0, 2:, 7].isnan().all() and got[3, :2].isnan().all()
+    got[0, 2:, 7], got[3, :2] = clean[0, 2:, 7], clean[3, :2]
+    assert torch.equal(got, clean)
