@@ -161,17 +161,23 @@ __device__ __forceinline__ int sequence_length(const PagedArgs &a, int b) {
   return n < 0 ? 0 : n < a.max_tokens ? (int)n : a.max_tokens;
 }
 
+// The running maximum of a row that had tokens, but scores of -inf alone: below every other one, but no -inf, which says
+// that no token counted.  (Their softmax is 0 / 0.)
+constexpr float kAllMinusInf = -3.4028234663852886e38f;
+// The output of a row whose weights add up to nothing.
+__device__ __forceinline__ float no_weights(float m) { return m == -INFINITY ? 0.f : __builtin_nanf(""); }
+
 // The sums of a row over a stretch of its sequence, or over all of it (`whole`: then the output).
 // `out_row`: b * n_q_heads + query head.
 template <typename T, typename Tile, int kJ>
 __device__ __forceinline__ void write_sums(const PagedArgs &a, bool whole, int64_t out_row, int64_t part_row, int kD,
                                            int r, int j0, float m, float l, float v_scale, const float *at) {
   if (whole) {
-    const float by = l > 0.f ? v_scale / l : l == 0.f ? 0.f : l;   // (no token, or NaN)
+    const float by = v_scale / l;
     char *o = a.out + out_row * kD * T::kBytes;
     float f[kJ];
 #pragma unroll
-    for (int j = 0; j < kJ; ++j) f[j] = l == 0.f ? 0.f : at[j] * by;
+    for (int j = 0; j < kJ; ++j) f[j] = l == 0.f ? no_weights(m) : at[j] * by;
     if constexpr (T::kBytes == 2) {
       uint32_t w[kJ / 2];
 #pragma unroll
@@ -587,6 +593,17 @@ __global__ void __launch_bounds__(kPagedThreads, paged_resident(kD, KV::kBytes, 
       l[r] += __shfl_xor(l[r], 16, 64);
       l[r] += __shfl_xor(l[r], 32, 64);
     }
+    bool none = false;
+#pragma unroll
+    for (int r = 0; r < kM; ++r) none = none || m[r] == -INFINITY;
+    if (any && __any(none)) {   // (rare: whether a token counted is looked up again rather than carried along)
+      bool counted = false;
+      for (int t = first_tile(cur); t < cur.t1 && !counted; t += kUnit)
+        counted = __any(t + (lane & (kTokens - 1)) < cur.t1 && page_of(cur.b, t) >= 0);
+#pragma unroll
+      for (int r = 0; r < kM; ++r)
+        if (counted) m[r] = fmaxf(m[r], kAllMinusInf);
+    }
 
     // ---- the waves' sums together, sixteen rows and kJ channels of each slice at a time
     const bool whole = cur.from == 0 && cur.to == cur.units;
@@ -695,7 +712,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const PagedAr
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < kParts; ++i) t += sums[i][x];
-    store_elem<T>(a.out, out_row * kD + x, l == 0.f ? 0.f : t * (v_scale / l));
+    store_elem<T>(a.out, out_row * kD + x, l == 0.f ? no_weights(mx) : t * (v_scale / l));
   }
   if (threadIdx.x == 0 && a.lse != nullptr) a.lse[out_row] = l == 0.f ? -INFINITY : mx * kLn2 + logf(l);
 }

@@ -60,7 +60,8 @@ def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     :func:`append_kv_pages_`, head_dim 64, 96, 128 or 256; lengths (sequences,) int32 or int64, on the device: they
     include the token itself where its key was stored before.  ``scale``: head_dim ** -0.5 by default.  Returns a tensor
     like xq (``out`` if given); fills ``lse`` (sequences, heads) fp32, the natural logarithm of the softmax denominator.
-    A sequence of no tokens gets zeros (lse -inf), and tokens on pages that are none of the pool's do not count.
+    A sequence of no tokens gets zeros (lse -inf), and tokens on pages that are none of the pool's do not count; a query
+    whose scores are all -inf gets the definition's NaN (lse -inf).
     16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, by weights of 24 bits (bf16) or ones that
     are kept to 2^-20 of themselves or 2^-40 of the sequence's largest, whichever is more (fp16: an infinite value under a
     weight below 2^-29 of the largest may give NaN); fp32 ones are multiplied in fp32.  The same shapes and lengths give the

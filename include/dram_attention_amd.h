@@ -676,7 +676,8 @@ int da_paged_append(const void *args, size_t args_bytes, void *stream);
  * out[b, j] = softmax_t(q[b, j] . k_t * scale) v_t over the first lengths[b] tokens t of sequence b, whose keys and
  * values lie in the pages of da_paged_append; query head j reads kv head j / (n_q_heads / n_kv_heads).  8-bit keys and
  * values stand for themselves times their kv head's scale.  Lengths are clamped to 0 .. pages_per_sequence * page_size;
- * tokens on pages that are none of the pool's do not count; a query for which no token counts gets zeros (lse -inf).
+ * tokens on pages that are none of the pool's do not count; a query for which no token counts gets zeros (lse -inf), one
+ * whose tokens' scores are all -inf NaN (0 / 0; lse -inf).
  *   q         : (n_sequences, n_q_heads, head_dim), 16-byte aligned rows;  out: the same shape, contiguous, 16-byte aligned
  *   lse       : optional (n_sequences, n_q_heads) fp32, natural log of the softmax denominator
  *   workspace : da_paged_attention_workspace_bytes(args, args_bytes) bytes, 16-byte aligned, contents may be anything;

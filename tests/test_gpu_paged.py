@@ -707,3 +707,33 @@ def test_missing_values_stay_with_their_sequence_and_head(types):
     assert got[0, 2:, 7].isnan().all() and got[3, :2].isnan().all()
     got[0, 2:, 7], got[3, :2] = clean[0, 2:, 7], clean[3, :2]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (6, 2, 128), (40, 1, 128)], ids=str)
+@pytest.mark.parametrize("types", TYPES[:3], ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
+def test_scores_of_minus_infinity(types, heads):
+    """A sequence of which every token scores -inf has the definition's 0 / 0 and a denominator of 0; where others do not,
+    its tokens weigh nothing, as if they were not there.  A sequence without tokens has zeros."""
+    dtype, _ = types
+    lengths = [40, 40, 3000, 3000, 0, 700, 20]
+    args, _ = attention_case(gen(34), lengths, *heads, dtype)
+    q, kp, vp, table, lens = args
+    q[..., 0] = 1
+    rep = heads[0] // heads[1]
+    for b in (0, 2):                                            # all tokens, of kv head 0
+        kp[table[b, : -(-lengths[b] // 16)].long(), :, 0, 0] = -float("inf")
+    without = table.clone()
+    for b, pages in ((1, [0, 1]), (3, range(3, 150)), (5, [43]), (6, [])):     # whole pages, of all kv heads
+        for i in pages:
+            kp[int(table[b, i]), :, :, 0] = -float("inf")
+            without[b, i] = -1
+    lse, want_lse = torch.zeros(q.shape[:2], device=DEV), torch.zeros(q.shape[:2], device=DEV)
+    got = paged_decode_attention(*args, lse=lse)
+    want = paged_decode_attention(q, kp, vp, without, lens, lse=want_lse)
+    for b in (0, 2):
+        assert got[b, :rep].isnan().all() and (lse[b, :rep] == -math.inf).all()
+        assert not got[b, rep:].isnan().any() and lse[b, rep:].isfinite().all()
+    assert not got[4].any() and (lse[4] == -math.inf).all()
+    assert torch.equal(got[[1, 3, 4, 5, 6]], want[[1, 3, 4, 5, 6]]) and torch.equal(lse, want_lse)
+    assert torch.equal(got[:, rep:], want[:, rep:])
+    assert not got[[1, 3, 5, 6]].isnan().any()
