@@ -20,6 +20,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -507,6 +508,10 @@ void not_for_gradients(std::initializer_list<const at::Tensor *> all, const char
     for (const at::Tensor *t : all)
       TORCH_CHECK(!t || !t->requires_grad(), what, " has no gradient: call it under torch.no_grad()");
 }
+// A dual tensor's tangent is no operand of the kernels: refused where forward mode is on, under torch.no_grad too.
+void not_forward_mode(const char *what) {
+  TORCH_CHECK(!torch::autograd::ForwardADLevel::try_get_by_idx(0), what, " has no forward-mode derivative");
+}
 // What a call writes into, autograd knows as changed.
 void changed(const at::Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -683,6 +688,7 @@ PyObject *rotate(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   TORCH_CHECK_TYPE(turn.freqs != nullptr, "freqs must be a tensor");
   const bool in_place = in.integer() != 0;
   TORCH_CHECK_TYPE(in.ok, "rotate: bad argument");
+  not_forward_mode(in_place ? "rotate_" : "rotate");
   if (xk) {
     TORCH_CHECK_TYPE(xk->scalar_type() == xq.scalar_type(), "xk is ", xk->scalar_type(), " but xq is ", xq.scalar_type());
     TORCH_CHECK_VALUE(xk->dim() == dims && xk->size(-1) == D && xk->size(dims - 3) == S && (dims == 3 || xk->size(0) == B),
@@ -787,6 +793,7 @@ PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   const Turn turn = read_turn(in, D);
   const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
   TORCH_CHECK_TYPE(in.ok, "append_kv_pages_: bad argument");
+  not_forward_mode("append_kv_pages_");
   TORCH_CHECK_VALUE(xk.dim() == 3 && xk.size(1) == H && xk.size(2) == D && xv.sizes() == xk.sizes(), "xk ", xk.sizes(),
                     " and xv ", xv.sizes(), " must both be (tokens, ", H, ", ", D, ") as the pages are");
   const int64_t T = xk.size(0);
@@ -878,6 +885,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
   const at::Tensor *out_given = plain_or_none(in.next(), "out"), *lse = plain_or_none(in.next(), "lse");
   TORCH_CHECK_TYPE(in.ok, "paged_decode_attention: bad argument");
+  not_forward_mode("paged_decode_attention");
   TORCH_CHECK_VALUE(xq.dim() == 3 && xq.size(0) == B && xq.size(2) == D && xq.size(1) > 0 && xq.size(1) % H == 0, "xq ",
                     xq.sizes(), " must be (", B, " sequences, a multiple of ", H, " heads, ", D, ")");
   const int64_t Hq = xq.size(1);

@@ -11,7 +11,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -101,8 +100,6 @@ def rotate(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, f
     ``factor`` are :func:`rotary_frequencies`'s.  bf16, fp16 or fp32 with any strides; products in fp32, rounded once.
     A call with gradients that is captured into a graph refuses leaves that an eager graph still holds.
     """
-    if forward_ad._current_level >= 0:
-        raise RuntimeError("rotate has no forward-mode derivative")
     return _lib.host().rotate(xq, xk, positions, freqs, layout_code(layout), float(factor), 0)
 
 

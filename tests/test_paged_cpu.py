@@ -275,3 +275,32 @@ def test_division_by_multiplication():
         assert m < 1 << 32
         for n in [0, 1, d - 1, d, d + 1, (1 << 31) - 1, (1 << 31) - d if d < 1 << 31 else 0] + [rng.randrange(1 << 31) for _ in range(50)]:
             assert ((m * n >> 32) + n) >> l == n // d, (n, d)
+
+
+def calls_of_a_batch():
+    """Every call as it would be made, on the CPU, where all that is wrong with it is the device."""
+    x = torch.zeros(3, 4, 64)
+    return {
+        "rotate": lambda x=x: rotate(**rotate_operands(xq=x[None].expand(2, 3, 4, 64))),
+        "rotate_": lambda x=x: rotate_(x, None, torch.arange(3), torch.zeros(32, dtype=torch.float64)),
+        "append_kv_pages_": lambda x=X: append_kv_pages_(x, X, positions=I, **pages_on_cpu()),
+        "paged_decode_attention": lambda x=x: paged_decode_attention(x, lengths=I, **pages_on_cpu()),
+    }
+
+
+@pytest.mark.parametrize("name", list(calls_of_a_batch()))
+def test_no_call_drops_a_tangent(name):
+    """Under torch.no_grad too, which leaves forward mode on."""
+    import torch.autograd.forward_ad as fwad
+
+    call = calls_of_a_batch()[name]
+    with fwad.dual_level():
+        x = X if name == "append_kv_pages_" else torch.zeros(3, 4, 64)
+        dual = fwad.make_dual(x.clone(), torch.ones_like(x))
+        for operand in (dual, x):
+            with pytest.raises(RuntimeError, match=f"^{name} has no forward-mode"):
+                call(operand)
+            with torch.no_grad(), pytest.raises(RuntimeError, match=f"^{name} has no forward-mode"):
+                call(operand)
+    with pytest.raises(RuntimeError, match="GPU"):
+        call()
