@@ -14,8 +14,11 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <hip/hip_runtime_api.h>
@@ -512,6 +515,15 @@ void not_for_gradients(std::initializer_list<const at::Tensor *> all, const char
 void not_forward_mode(const char *what) {
   TORCH_CHECK(!torch::autograd::ForwardADLevel::try_get_by_idx(0), what, " has no forward-mode derivative");
 }
+// A tracer would write down the outputs' allocation and nothing else: its program would return memory as it was.
+// (Dispatch modes that count, log or keep operators are no tracers: what a call returns under them is right.)
+void not_traced(const char *what) {
+  using namespace c10::impl;
+  TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled() &&                              // torch.jit.trace
+                  !TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) &&      // make_fx
+                  !tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch),        // make_fx ahead of autograd
+              what, " cannot be traced: a tracer sees none of its kernels");
+}
 // What a call writes into, autograd knows as changed.
 void changed(const at::Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -689,6 +701,7 @@ PyObject *rotate(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   const bool in_place = in.integer() != 0;
   TORCH_CHECK_TYPE(in.ok, "rotate: bad argument");
   not_forward_mode(in_place ? "rotate_" : "rotate");
+  not_traced(in_place ? "rotate_" : "rotate");
   if (xk) {
     TORCH_CHECK_TYPE(xk->scalar_type() == xq.scalar_type(), "xk is ", xk->scalar_type(), " but xq is ", xq.scalar_type());
     TORCH_CHECK_VALUE(xk->dim() == dims && xk->size(-1) == D && xk->size(dims - 3) == S && (dims == 3 || xk->size(0) == B),
@@ -794,6 +807,7 @@ PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
   TORCH_CHECK_TYPE(in.ok, "append_kv_pages_: bad argument");
   not_forward_mode("append_kv_pages_");
+  not_traced("append_kv_pages_");
   TORCH_CHECK_VALUE(xk.dim() == 3 && xk.size(1) == H && xk.size(2) == D && xv.sizes() == xk.sizes(), "xk ", xk.sizes(),
                     " and xv ", xv.sizes(), " must both be (tokens, ", H, ", ", D, ") as the pages are");
   const int64_t T = xk.size(0);
@@ -886,6 +900,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   const at::Tensor *out_given = plain_or_none(in.next(), "out"), *lse = plain_or_none(in.next(), "lse");
   TORCH_CHECK_TYPE(in.ok, "paged_decode_attention: bad argument");
   not_forward_mode("paged_decode_attention");
+  not_traced("paged_decode_attention");
   TORCH_CHECK_VALUE(xq.dim() == 3 && xq.size(0) == B && xq.size(2) == D && xq.size(1) > 0 && xq.size(1) % H == 0, "xq ",
                     xq.sizes(), " must be (", B, " sequences, a multiple of ", H, " heads, ", D, ")");
   const int64_t Hq = xq.size(1);

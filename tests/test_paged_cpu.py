@@ -304,3 +304,26 @@ def test_no_call_drops_a_tangent(name):
                 call(operand)
     with pytest.raises(RuntimeError, match="GPU"):
         call()
+
+
+@pytest.mark.parametrize("name", list(calls_of_a_batch()))
+def test_no_call_is_traced(name):
+    """What a tracer would keep of a call is its output's allocation; modes that only watch are no tracers."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    call = calls_of_a_batch()[name]
+    x = X if name == "append_kv_pages_" else torch.zeros(3, 4, 64)
+
+    def traced(x):
+        with pytest.raises(RuntimeError, match=f"^{name} cannot be traced"):
+            call(x)
+        return x + 1
+
+    make_fx(traced)(x)
+    make_fx(traced, pre_dispatch=True)(x)
+    torch.jit.trace(traced, x, check_trace=False)
+    with FlopCounterMode(display=False), pytest.raises(RuntimeError, match="GPU"):
+        call(x)
+    with torch.device("cpu"), pytest.raises(RuntimeError, match="GPU"):
+        call(x)
