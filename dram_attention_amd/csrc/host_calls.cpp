@@ -662,6 +662,8 @@ struct Turned : torch::autograd::Function<Turned> {
   }
 
   static Variables backward(Context *ctx, Variables grads) {
+    not_forward_mode("rotate's gradient");
+    not_traced("rotate's gradient");
     const Variables saved = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();
     const double factor = ctx->saved_data["factor"].toDouble();

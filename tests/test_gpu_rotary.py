@@ -296,3 +296,36 @@ def test_refusals_that_need_a_gpu():
         rotate_(torch.zeros(4, 2, 128, device=DEV)[..., ::2], None, positions, freqs)
     with pytest.raises(RuntimeError, match="no gradient"):
         rotate_(x.clone().requires_grad_(), None, positions, freqs)
+
+
+def test_the_gradient_drops_no_tangent_and_is_not_traced():
+    """A backward pass of an eager graph under forward mode or a tracer; the same graph is taken without them."""
+    import torch.autograd.forward_ad as fwad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    g = gen(11)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(5, device=DEV)
+    q = randn(g, 5, 2, 64, dtype=torch.float32).requires_grad_()
+    gr = randn(g, 5, 2, 64, dtype=torch.float32)
+    y, _ = rotate(q, None, positions, freqs)
+
+    def back(x):
+        return torch.autograd.grad(y, (q,), x, retain_graph=True)[0]
+
+    with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        back(fwad.make_dual(gr, torch.ones_like(gr)))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(back)(gr)
+    check(back(gr), gr, -positions, freqs, "interleaved")
+
+
+def test_transforms_are_refused():
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions, x = torch.arange(5, device=DEV), torch.ones(3, 5, 2, 64, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda q: rotate(q, None, positions, freqs)[0])(x)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda q: rotate(q, None, positions, freqs)[0].sum())(x)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: rotate(q, None, positions, freqs)[0], (x,), (x,))
