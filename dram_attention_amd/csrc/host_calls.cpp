@@ -658,6 +658,9 @@ struct Turned : torch::autograd::Function<Turned> {
     ctx->saved_data["how"] = (int64_t)(half | inverse << 1 | (int)k.has_value() << 2);
     ctx->saved_data["factor"] = factor;
     Pair y = turn_rows(q, k ? *k : at::Tensor(), positions, {&freqs, half, factor}, inverse, false);
+    // (each output wants a gradient if its own input does)
+    if (k && !q.requires_grad()) ctx->mark_non_differentiable({y.q});
+    if (k && !k->requires_grad()) ctx->mark_non_differentiable({y.k});
     return k ? Variables{y.q, y.k} : Variables{y.q};
   }
 

@@ -329,3 +329,25 @@ def test_transforms_are_refused():
         torch.func.grad(lambda q: rotate(q, None, positions, freqs)[0].sum())(x)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda q: rotate(q, None, positions, freqs)[0], (x,), (x,))
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+def test_an_output_wants_a_gradient_if_its_input_does(layout):
+    g = gen(12)
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(5, device=DEV)
+    q, k = randn(g, 5, 4, 64, dtype=torch.float32), randn(g, 5, 2, 64, dtype=torch.float32)
+    want = rotate(q, k, positions, freqs, layout=layout)
+    for wants in ((True, False), (False, True), (True, True)):
+        x = [t.clone().requires_grad_(w) for t, w in zip((q, k), wants)]
+        y = rotate(*x, positions, freqs, layout=layout)
+        assert [t.requires_grad for t in y] == list(wants) and [t.is_leaf for t in y] == [not w for w in wants]
+        assert all(torch.equal(a, b) for a, b in zip(y, want))
+        gr = [randn(g, *t.shape, dtype=t.dtype).requires_grad_() for t in y]
+        leaves, outs = [t for t in x if t.requires_grad], [t for t in y if t.requires_grad]
+        back = torch.autograd.grad(outs, leaves, [r for r, t in zip(gr, y) if t.requires_grad], create_graph=True)
+        for d, r in zip(back, [r for r, t in zip(gr, y) if t.requires_grad]):
+            check(d, r, -positions, freqs, layout)
+            v = randn(g, *d.shape, dtype=d.dtype)
+            again, = torch.autograd.grad(d, (r,), v, retain_graph=True)
+            check(again, v, positions, freqs, layout)
