@@ -26,7 +26,9 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <string>
 #include <vector>
@@ -530,6 +532,33 @@ void changed(const at::Tensor &t) {
 }
 int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 bool dense_rows(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
+// Whether two tensors of the same sizes and strides have a byte in common, exactly: they lie `apart` bytes from each other,
+// and have if differences of their indices make that up to less than an element.  Axes go from the longest stride to the
+// shortest, with the differences that the shorter ones can still make up: one or two an axis, or more where strides are
+// shorter than what lies within them (then at most `budget` are looked at, and the tensors are taken to meet).
+struct Axis {
+  int64_t stride, most;   // bytes; largest difference of its indices
+};
+bool made_up(const Axis *axes, size_t n, int64_t apart, int64_t element, int &budget) {
+  if (n == 0) return std::abs(apart) < element;
+  int64_t within = element - 1;
+  for (size_t i = 1; i < n; ++i) within += axes[i].stride * axes[i].most;
+  auto floored = [](int64_t x, int64_t d) { return x / d - (x % d < 0); };
+  const int64_t s = axes[0].stride, first = std::max(-axes[0].most, -floored(within + apart, s)),
+                last = std::min(axes[0].most, floored(within - apart, s));
+  for (int64_t by = first; by <= last; ++by)
+    if (--budget < 0 || made_up(axes + 1, n - 1, apart + by * s, element, budget)) return true;
+  return false;
+}
+bool meet(const at::Tensor &a, const at::Tensor &b) {
+  if (a.numel() == 0) return false;
+  std::vector<Axis> axes;
+  for (int64_t d = 0; d < a.dim(); ++d)
+    if (a.size(d) > 1 && a.stride(d) > 0) axes.push_back({a.stride(d) * (int64_t)a.element_size(), a.size(d) - 1});
+  std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.stride > y.stride; });
+  int budget = 4096;
+  return made_up(axes.data(), axes.size(), (const char *)b.data_ptr() - (const char *)a.data_ptr(), a.element_size(), budget);
+}
 // Rows as the kernels read them: the last axis dense, and where `vectors` 16-byte aligned.  (A gradient may be a lazy
 // view of what its memory holds.)
 at::Tensor rows_of(const at::Tensor &t, bool vectors) {
@@ -833,6 +862,7 @@ PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   not_for_gradients({&xk, &xv, xq, &pages.k, &pages.v}, "append_kv_pages_");
   for (const at::Tensor *t : {&pages.k, &pages.v})
     TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "pages must not share memory");
+  TORCH_CHECK_VALUE(!meet(pages.k, pages.v), "k_pages and v_pages share memory");
   on_device_of(xk, {{&xv, "xv"}, {&pages.k, "k_pages"}, {&pages.v, "v_pages"}, {&pages.table, "page_table"},
                     {&positions, "positions"}, {sequences, "sequences"}, {xq, "xq"}, {turn.freqs, "freqs"},
                     {k_scale, "k_scale"}, {v_scale, "v_scale"}});

@@ -36,8 +36,8 @@ def append_kv_pages_(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, 
     """Store keys, turned by their positions on the way, and values in their sequences' pages; returns the turned
     queries (None without ``xq``).
 
-    xk, xv (tokens, kv heads, head_dim); k_pages, v_pages (pages, page_size, kv heads, head_dim) of the same strides;
-    page_table (sequences, pages) and positions (tokens,) int32 or int64.  Token t is of row sequences[t] of the table,
+    xk, xv (tokens, kv heads, head_dim); k_pages, v_pages (pages, page_size, kv heads, head_dim) of the same strides
+    that share no memory; page_table (sequences, pages) and positions (tokens,) int32 or int64.  Token t is of row sequences[t] of the table,
     or of row t without ``sequences`` (a decode step), and goes to slot p % page_size of page page_table[row, p //
     page_size], p = positions[t].  Tokens of a call have places of their own.  Not stored: a token whose position is
     negative (padding) or beyond its row of the table, whose sequence is none of the table's, or whose page number is

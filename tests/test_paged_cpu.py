@@ -327,3 +327,45 @@ def test_no_call_is_traced(name):
         call(x)
     with torch.device("cpu"), pytest.raises(RuntimeError, match="GPU"):
         call(x)
+
+
+def append_into(k, v):
+    d, heads = k.shape[-1], k.shape[2]
+    x = torch.zeros(3, heads, d, dtype=k.dtype)
+    append_kv_pages_(x, x, k, v, torch.zeros(3, 2, dtype=torch.int32), I)
+
+
+def test_append_refuses_pools_that_share_memory():
+    """Keys and values would race for the same bytes; pools that only lie between each other are taken."""
+    base = torch.zeros(13, 32, 4, 64)
+    k, v = kv_pages(6, 16, 2, 64, dtype=torch.float32, device="cpu")
+    for a, b in ((k, k), (k, k[:]), (v, v.view(v.shape)), (base[:6], base[5:11]), (base[:6], base[:6]),
+                 (base[:6, :16], base[:6, 15:31]), (base[:6, :, :2], base[:6, :, 1:3]),
+                 (base[:6, :, :, :32], base[:6, :, :, 16:48]), (base[::2], base[::2])):
+        with pytest.raises(ValueError, match="share memory"):
+            append_into(a, b)
+    for a, b in ((k, v), (v, k), (base[:6], base[6:12]), (base[6:12], base[:6]), (base[:12:2], base[1:13:2]),
+                 (base[:6, :16], base[:6, 16:]), (base[:6, ::2], base[:6, 1::2]), (base[:6, :, ::2], base[:6, :, 1::2]),
+                 (base[:6, :, :, :32], base[:6, :, :, 32:]), (base[:0], base[:0]), (base[:6], base.clone()[:6])):
+        with pytest.raises(RuntimeError, match="GPU"):
+            append_into(a, b)
+
+
+def test_pools_that_share_memory_are_found_exactly():
+    """Against the sets of elements, over views of any strides of one buffer."""
+    import random
+
+    rng = random.Random(3)
+    buffer = torch.zeros(4000, dtype=torch.bfloat16)
+    met = 0
+    for _ in range(400):
+        sizes = [rng.randint(1, 4), rng.randint(1, 4), rng.randint(1, 3), rng.choice([2, 3, 8])]
+        strides = [rng.choice([1, 3, 8, 12, 16, 40, 64, 200]) for _ in range(3)] + [1]
+        offsets = [rng.randint(0, 200), rng.randint(0, 200)]
+        pools = [buffer.as_strided(sizes, strides, at) for at in offsets]
+        sets = [set(torch.arange(4000).as_strided(sizes, strides, at).flatten().tolist()) for at in offsets]
+        shared = bool(sets[0] & sets[1])
+        met += shared
+        with pytest.raises(ValueError if shared else RuntimeError, match="share memory" if shared else "GPU"):
+            append_into(*pools)
+    assert 100 < met < 300
