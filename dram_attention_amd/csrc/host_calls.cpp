@@ -20,6 +20,7 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/Exceptions.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -539,6 +540,7 @@ bool dense_rows(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) ==
 struct Axis {
   int64_t stride, most;   // bytes; largest difference of its indices
 };
+using Axes = c10::SmallVector<Axis, 4>;
 bool made_up(const Axis *axes, size_t n, int64_t apart, int64_t element, int &budget) {
   if (n == 0) return std::abs(apart) < element;
   int64_t within = element - 1;
@@ -550,14 +552,42 @@ bool made_up(const Axis *axes, size_t n, int64_t apart, int64_t element, int &bu
     if (--budget < 0 || made_up(axes + 1, n - 1, apart + by * s, element, budget)) return true;
   return false;
 }
-bool meet(const at::Tensor &a, const at::Tensor &b) {
-  if (a.numel() == 0) return false;
-  std::vector<Axis> axes;
-  for (int64_t d = 0; d < a.dim(); ++d)
-    if (a.size(d) > 1 && a.stride(d) > 0) axes.push_back({a.stride(d) * (int64_t)a.element_size(), a.size(d) - 1});
+Axes axes_of(const at::Tensor &t) {
+  Axes axes;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) > 0) axes.push_back({t.stride(d) * (int64_t)t.element_size(), t.size(d) - 1});
   std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.stride > y.stride; });
-  int budget = 4096;
+  return axes;
+}
+constexpr int kMostLookedAt = 4096;
+bool meet(const at::Tensor &a, const at::Tensor &b) {
+  if (a.numel() == 0 || a.is_meta()) return false;
+  const Axes axes = axes_of(a);
+  int budget = kMostLookedAt;
   return made_up(axes.data(), axes.size(), (const char *)b.data_ptr() - (const char *)a.data_ptr(), a.element_size(), budget);
+}
+// Whether a tensor has a byte in memory of `length` bytes that its first element is `at` bytes behind, in the same way.
+bool reached(const Axis *axes, size_t n, int64_t at, int64_t element, int64_t length, int &budget) {
+  int64_t within = element - 1;   // (to the last byte, behind the axes from the second on)
+  for (size_t i = 1; i < n; ++i) within += axes[i].stride * axes[i].most;
+  const int64_t end = at + within + (n ? axes[0].stride * axes[0].most : 0);
+  if (end < 0 || at >= length) return false;
+  if (n == 0 || at >= 0 || end < length) return true;   // (its first or last byte is there)
+  const int64_t s = axes[0].stride, first = std::max<int64_t>(0, (-within - at + s - 1) / s),
+                last = std::min(axes[0].most, (length - 1 - at) / s);
+  for (int64_t by = first; by <= last; ++by)
+    if (--budget < 0 || reached(axes + 1, n - 1, at + by * s, element, length, budget)) return true;
+  return false;
+}
+bool reaches(const at::Tensor &t, const at::Tensor &memory) {   // (`memory` is contiguous)
+  if (t.numel() == 0 || memory.numel() == 0 || t.is_meta() || memory.is_meta()) return false;
+  const int64_t at = (const char *)t.data_ptr() - (const char *)memory.data_ptr(), length = memory.nbytes();
+  int64_t extent = t.element_size();
+  for (int64_t d = 0; d < t.dim(); ++d) extent += (t.size(d) - 1) * t.stride(d) * (int64_t)t.element_size();
+  if (at >= length || at + extent <= 0) return false;
+  const Axes axes = axes_of(t);
+  int budget = kMostLookedAt;
+  return reached(axes.data(), axes.size(), at, t.element_size(), length, budget);
 }
 // Rows as the kernels read them: the last axis dense, and where `vectors` 16-byte aligned.  (A gradient may be a lazy
 // view of what its memory holds.)
@@ -949,6 +979,12 @@ PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
     TORCH_CHECK_VALUE(lse->scalar_type() == at::kFloat && is_shape(*lse, {B, Hq}) && lse->is_contiguous(),
                       "lse must be contiguous float32 of shape (sequences, heads)");
   not_for_gradients({&xq, &pages.k, &pages.v, k_scale, v_scale, out_given}, "paged_decode_attention");
+  // (a workgroup has a sequence's queries before it writes there, or the launch behind writes: out may be xq itself)
+  for (const at::Tensor *to : {out_given, lse})
+    for (const at::Tensor *from : {&xq, &pages.k, &pages.v, &pages.table, &lengths, k_scale, v_scale, lse})
+      TORCH_CHECK_VALUE(!to || !from || from == to || !reaches(*from, *to) ||
+                            (to == out_given && from == &xq && xq.data_ptr() == to->data_ptr() && xq.is_contiguous()),
+                        to == lse ? "lse" : "out", " shares memory with another operand");
   on_device_of(xq, {{&pages.k, "k_pages"}, {&pages.v, "v_pages"}, {&pages.table, "page_table"}, {&lengths, "lengths"},
                     {k_scale, "k_scale"}, {v_scale, "v_scale"}, {out_given, "out"}, {lse, "lse"}});
   const c10::DeviceGuard guard(xq.device());

@@ -37,11 +37,11 @@ def append_kv_pages_(xk: torch.Tensor, xv: torch.Tensor, k_pages: torch.Tensor, 
     queries (None without ``xq``).
 
     xk, xv (tokens, kv heads, head_dim); k_pages, v_pages (pages, page_size, kv heads, head_dim) of the same strides
-    that share no memory; page_table (sequences, pages) and positions (tokens,) int32 or int64.  Token t is of row sequences[t] of the table,
-    or of row t without ``sequences`` (a decode step), and goes to slot p % page_size of page page_table[row, p //
-    page_size], p = positions[t].  Tokens of a call have places of their own.  Not stored: a token whose position is
-    negative (padding) or beyond its row of the table, whose sequence is none of the table's, or whose page number is
-    none of the pool's; its query is turned all the same.
+    that share no memory; page_table (sequences, pages) and positions (tokens,) int32 or int64.  Token t is of row
+    sequences[t] of the table, or of row t without ``sequences`` (a decode step), and goes to slot p % page_size of page
+    page_table[row, p // page_size], p = positions[t].  Tokens of a call have places of their own, which no operand of
+    the call is a view of.  Not stored: a token whose position is negative (padding) or beyond its row of the table,
+    whose sequence is none of the table's, or whose page number is none of the pool's; its query is turned all the same.
     xq (tokens, heads, head_dim), ``freqs`` (None: nothing turns), ``layout``, ``factor``: as of :func:`rotate`.
     k_scale, v_scale (kv heads,) float32 above 0: 8-bit pages hold a key or value divided by its head's, clamped to 448
     and rounded to nearest; without them 1.
@@ -59,7 +59,8 @@ def paged_decode_attention(xq: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     xq (sequences, heads, head_dim), heads a multiple of the kv heads; pages and page_table as of
     :func:`append_kv_pages_`, head_dim 64, 96, 128 or 256; lengths (sequences,) int32 or int64, on the device: they
     include the token itself where its key was stored before.  ``scale``: head_dim ** -0.5 by default.  Returns a tensor
-    like xq (``out`` if given); fills ``lse`` (sequences, heads) fp32, the natural logarithm of the softmax denominator.
+    like xq (``out`` if given, which may be a contiguous xq itself); fills ``lse`` (sequences, heads) fp32, the natural
+    logarithm of the softmax denominator.  Neither shares memory with another operand.
     A sequence of no tokens gets zeros (lse -inf), and tokens on pages that are none of the pool's do not count; a query
     whose scores are all -inf gets the definition's NaN (lse -inf).
     16-bit and 8-bit keys and values are multiplied exactly and summed in fp32, by weights of 24 bits (bf16) or ones that

@@ -678,7 +678,8 @@ int da_paged_append(const void *args, size_t args_bytes, void *stream);
  * values stand for themselves times their kv head's scale.  Lengths are clamped to 0 .. pages_per_sequence * page_size;
  * tokens on pages that are none of the pool's do not count; a query for which no token counts gets zeros (lse -inf), one
  * whose tokens' scores are all -inf NaN (0 / 0; lse -inf).
- *   q         : (n_sequences, n_q_heads, head_dim), 16-byte aligned rows;  out: the same shape, contiguous, 16-byte aligned
+ *   q         : (n_sequences, n_q_heads, head_dim), 16-byte aligned rows
+ *   out       : the same shape, contiguous, 16-byte aligned; q itself, or (as lse) memory of its own
  *   lse       : optional (n_sequences, n_q_heads) fp32, natural log of the softmax denominator
  *   workspace : da_paged_attention_workspace_bytes(args, args_bytes) bytes, 16-byte aligned, contents may be anything;
  *               not shared by calls that may run at the same time

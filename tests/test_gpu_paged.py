@@ -737,3 +737,14 @@ def test_scores_of_minus_infinity(types, heads):
     assert torch.equal(got[[1, 3, 4, 5, 6]], want[[1, 3, 4, 5, 6]]) and torch.equal(lse, want_lse)
     assert torch.equal(got[:, rep:], want[:, rep:])
     assert not got[[1, 3, 5, 6]].isnan().any()
+
+
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x).replace("torch.", "") for x in t))
+@pytest.mark.parametrize("lengths", [[40, 0, 300, 512], [3000, 1, 0, 700, 128, 5000, 17, 2]], ids=str)
+def test_the_output_may_be_the_queries(types, lengths):
+    dtype, cache = types
+    for heads in ((4, 2, 64), (33, 1, 128), (24, 8, 256)):
+        args, scales = attention_case(gen(35), lengths, *heads, dtype, cache)
+        want = paged_decode_attention(*args, **scales)
+        q = args[0].clone()
+        assert paged_decode_attention(q, *args[1:], **scales, out=q) is q and torch.equal(q, want)

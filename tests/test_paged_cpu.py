@@ -369,3 +369,45 @@ def test_pools_that_share_memory_are_found_exactly():
         with pytest.raises(ValueError if shared else RuntimeError, match="share memory" if shared else "GPU"):
             append_into(*pools)
     assert 100 < met < 300
+
+
+def test_attention_refuses_to_write_over_what_it_reads():
+    buffer = torch.zeros(1 << 16)
+    k, v = buffer[: 6 * 16 * 2 * 64 * 2].view(6, 2, 16, 2, 64).permute(0, 2, 1, 3, 4).unbind(3)
+    free = buffer[6 * 16 * 2 * 64 * 2:]
+    q, lse, out = free[:768].view(3, 4, 64), free[768:780].view(3, 4), free[1024:1792].view(3, 4, 64)
+    table, lengths = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+
+    def call(**more):
+        paged_decode_attention(**{**dict(xq=q, k_pages=k, v_pages=v, page_table=table, lengths=lengths), **more})
+
+    as_ints = free[768:780].view(torch.int32)
+    for more, what in (({"out": free[16:784].view(3, 4, 64)}, "out"), ({"out": buffer[64:832].view(3, 4, 64)}, "out"),
+                       ({"out": out, "lse": free[1790:1802].view(3, 4)}, "out"), ({"lse": free[767:779].view(3, 4)}, "lse"),
+                       ({"lse": lse, "lengths": as_ints[9:12]}, "lse"), ({"lse": lse, "page_table": as_ints[:6].view(3, 2)}, "lse"),
+                       ({"lse": buffer[:12].view(3, 4)}, "lse"),
+                       # (the same rows in another order)
+                       ({"xq": q.flip(0), "out": out}, None), ({"xq": free[:768].view(3, 64, 4).transpose(1, 2), "out": q}, "out"),
+                       ({"out": q}, None), ({"out": q[:]}, None), ({"out": out, "lse": lse}, None),
+                       ({"xq": free[: 2 * 768].view(3, 8, 64)[:, ::2], "out": free[2 * 768: 3 * 768].view(3, 4, 64)}, None)):
+        with pytest.raises(ValueError if what else RuntimeError, match=f"^{what} shares memory" if what else "GPU"):
+            call(**more)
+
+
+def test_memory_that_rows_reach_into_is_found_exactly():
+    """Against the sets of elements: logarithms in one buffer with queries of any strides, many with gaps that hold them."""
+    import random
+
+    rng = random.Random(4)
+    k, v = kv_pages(6, 16, 1, 2, dtype=torch.float32, device="cpu")
+    table, lengths, buffer, met = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(4000), 0
+    for _ in range(400):
+        strides, at, lse_at = [rng.choice([2, 5, 8, 16, 40, 200]) for _ in range(2)] + [1], rng.randint(0, 300), rng.randint(0, 400)
+        heads = rng.randint(1, 5)
+        rows = set(torch.arange(4000).as_strided((3, heads, 2), strides, at).flatten().tolist())
+        shared = bool(rows & set(range(lse_at, lse_at + 3 * heads)))
+        met += shared
+        with pytest.raises(ValueError if shared else RuntimeError, match="lse shares memory" if shared else "GPU"):
+            paged_decode_attention(buffer.as_strided((3, heads, 2), strides, at), k, v, table, lengths,
+                                   lse=buffer[lse_at: lse_at + 3 * heads].view(3, heads))
+    assert 40 < met < 360       # (both kinds)
