@@ -959,7 +959,8 @@ PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   if (scale_at != Py_None) {
     scale = PyFloat_AsDouble(scale_at);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite (got ", scale, ")");
+    // (the kernels have it in fp32, times log2 e)
+    TORCH_CHECK_VALUE(std::isfinite((float)scale * 1.4426950408889634f), "scale must be finite in fp32 (got ", scale, ")");
   }
   const at::Tensor *k_scale = read_scale(in.next(), "k_scale", pages), *v_scale = read_scale(in.next(), "v_scale", pages);
   const at::Tensor *out_given = plain_or_none(in.next(), "out"), *lse = plain_or_none(in.next(), "lse");

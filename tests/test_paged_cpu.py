@@ -411,3 +411,11 @@ def test_memory_that_rows_reach_into_is_found_exactly():
             paged_decode_attention(buffer.as_strided((3, heads, 2), strides, at), k, v, table, lengths,
                                    lse=buffer[lse_at: lse_at + 3 * heads].view(3, heads))
     assert 40 < met < 360       # (both kinds)
+
+
+@pytest.mark.parametrize("scale, fits", [(1e39, False), (-1e39, False), (3e38, False), (math.nan, False), (2.3e38, True),
+                                         (1e-60, True), (0.0, True), (-2.0, True)])
+def test_scales_that_fp32_does_not_hold_are_refused(scale, fits):
+    a = pages_on_cpu()
+    with pytest.raises(RuntimeError if fits else ValueError, match="GPU" if fits else "scale must be finite"):
+        paged_decode_attention(torch.zeros(3, 4, 64), lengths=I, scale=scale, **a)
