@@ -889,7 +889,7 @@ PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
                     T, " tokens");
   TORCH_CHECK_VALUE(sequences || T == pages.table.size(0), T, " tokens for the ", pages.table.size(0),
                     " sequences of the table: say which with sequences=");
-  not_for_gradients({&xk, &xv, xq, &pages.k, &pages.v}, "append_kv_pages_");
+  not_for_gradients({&xk, &xv, xq, &pages.k, &pages.v, k_scale, v_scale}, "append_kv_pages_");
   for (const at::Tensor *t : {&pages.k, &pages.v})
     TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "pages must not share memory");
   TORCH_CHECK_VALUE(!meet(pages.k, pages.v), "k_pages and v_pages share memory");
@@ -979,7 +979,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
   if (lse)
     TORCH_CHECK_VALUE(lse->scalar_type() == at::kFloat && is_shape(*lse, {B, Hq}) && lse->is_contiguous(),
                       "lse must be contiguous float32 of shape (sequences, heads)");
-  not_for_gradients({&xq, &pages.k, &pages.v, k_scale, v_scale, out_given}, "paged_decode_attention");
+  not_for_gradients({&xq, &pages.k, &pages.v, k_scale, v_scale, out_given, lse}, "paged_decode_attention");
   // (a workgroup has a sequence's queries before it writes there, or the launch behind writes: out may be xq itself)
   for (const at::Tensor *to : {out_given, lse})
     for (const at::Tensor *from : {&xq, &pages.k, &pages.v, &pages.table, &lengths, k_scale, v_scale, lse})

@@ -419,3 +419,17 @@ def test_scales_that_fp32_does_not_hold_are_refused(scale, fits):
     a = pages_on_cpu()
     with pytest.raises(RuntimeError if fits else ValueError, match="GPU" if fits else "scale must be finite"):
         paged_decode_attention(torch.zeros(3, 4, 64), lengths=I, scale=scale, **a)
+
+
+def test_scales_and_logarithms_that_want_gradients_are_refused():
+    a, h = pages_on_cpu(torch.float8_e4m3fn), X.bfloat16()
+    for name in ("k_scale", "v_scale"):
+        scale = torch.ones(2, requires_grad=True)
+        for call in (lambda: append_kv_pages_(h, h, positions=I, **{name: scale}, **a),
+                     lambda: paged_decode_attention(h, lengths=I, **{name: scale}, **a)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
+                call()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_decode_attention(h, lengths=I, lse=torch.zeros(3, 2, requires_grad=True), **a)
