@@ -38,7 +38,7 @@ def rotary_frequencies(rotary_dim: int, theta: float = 500000.0, scaling: dict |
     if not (math.isfinite(theta) and theta > 1):
         raise ValueError(f"theta must be above 1 (got {theta})")
     scaling = dict(scaling or {"type": None})
-    kind = scaling.pop("type")
+    kind = scaling.pop("type", None)
     base, factor = float(theta), 1.0
     pair = torch.arange(rotary_dim // 2, dtype=torch.float64)
 

@@ -433,3 +433,11 @@ def test_scales_and_logarithms_that_want_gradients_are_refused():
                 call()
     with pytest.raises(RuntimeError, match="no gradient"):
         paged_decode_attention(h, lengths=I, lse=torch.zeros(3, 2, requires_grad=True), **a)
+
+
+def test_a_scaling_without_a_type_is_refused():
+    with pytest.raises(ValueError, match="factor"):
+        freqs_of(8, 1e4, {"factor": 2.0})
+    given = {"type": "linear", "factor": 2.0}
+    freqs_of(8, 1e4, given)
+    assert given == {"type": "linear", "factor": 2.0}
