@@ -724,7 +724,9 @@ struct Turned : torch::autograd::Function<Turned> {
   }
 
   static Variables backward(Context *ctx, Variables grads) {
-    not_forward_mode("rotate's gradient");
+    // (gradients without a tangent are taken where forward mode is on for something else)
+    for (const at::Tensor &g : grads)
+      TORCH_CHECK(!g.defined() || !g._fw_grad(0).defined(), "rotate's gradient has no forward-mode derivative");
     not_traced("rotate's gradient");
     const Variables saved = ctx->get_saved_variables();
     const int64_t how = ctx->saved_data["how"].toInt();

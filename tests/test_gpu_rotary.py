@@ -315,6 +315,8 @@ def test_the_gradient_drops_no_tangent_and_is_not_traced():
 
     with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         back(fwad.make_dual(gr, torch.ones_like(gr)))
+    with fwad.dual_level():
+        check(back(gr), gr, -positions, freqs, "interleaved")
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(back)(gr)
     check(back(gr), gr, -positions, freqs, "interleaved")
