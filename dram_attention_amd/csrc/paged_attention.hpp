@@ -2,7 +2,8 @@
 //
 //   out[b, j] = sum_t w_t v_t / sum_t w_t,  w_t = exp(q[b, j] . k_t * scale - m),  m = the running maximum
 //
-// Bound: HBM (128K tokens of 32/8 heads of 128 in bf16 83 us = 6.4 TB/s, 16 sequences of up to that 712).  Every key and
+// Bound: HBM (16 sequences of up to 128K tokens of 64/8 heads of 128 in bf16 714 us = 6.4 TB/s, one of 32/8 heads 88 =
+// 5.8-6.1 TB/s, the first loads and the uneven end of 512 workgroups among it).  Every key and
 // value is read once for all the query heads that share it, up to 32; a group's query rows are padded to 16 so that both products are 16x16 matrix instructions, which cost next to nothing beside the loads.
 //
 // Split: the sequences of a kv head are laid end to end, in units of a tile for each of the four waves, and every workgroup takes
@@ -43,8 +44,8 @@ constexpr int paged_resident(int head_dim, int bytes, int sixteens) {
          : head_dim == 128 || bytes == 1                     ? 2
                                                              : 1;
 }
-// Sixteens of query rows that share a wave's keys and values, where a kv head has more: 64/2 heads over 1 GB 176 us
-// instead of 216 as two workgroups, 64/1 234 instead of 354.
+// Sixteens of query rows that share a wave's keys and values, where a kv head has more: 64/2 heads of 128 over 1 GB 193
+// us instead of 239 as two workgroups, 64/1 282 instead of 381.
 constexpr int paged_sixteens(int head_dim, int bytes, int rep) {
   return rep > 16 && head_dim <= 128 && bytes < 4 ? 2 : 1;
 }
@@ -730,10 +731,11 @@ template <typename T, typename KV, int kD>
 int launch_paged_dim(const PagedArgs &a, hipStream_t s) {
   const unsigned head_groups = (unsigned)(a.n_kv_heads * a.groups);
   const unsigned blocks = head_groups * (unsigned)(a.shares == 0 ? a.n_seqs : a.shares);
-  // Keys and values that are read once come by streaming where their rows are whole lines: 137 instead of 154 us for 834 MB
-  // of e4m3 rows of 128, 88 instead of 99 for 128K tokens of bf16 ones, the same for fp32 ones of 256.  Rows that share
-  // lines are read faster through the caches (bf16 ones of 96: 191 instead of 211 us for 1 GB, e4m3 ones of 64: 195, 220), and
-  // so are those that several groups of query heads read (two of 16 of 64/2 heads of 128: 216 instead of 278).
+  // Keys and values that are read once come by streaming where their rows are whole lines: 141 instead of 153 us for 800 MB
+  // of e4m3 rows of 128, 94 instead of 104 for 128K tokens of bf16 ones, 146 instead of 152 for 800 MB of fp32 ones (of 256
+  // 295 instead of 285 for 1.6 GB).  Rows that share lines are read faster through the caches (bf16 ones of 96: 223 instead
+  // of 261 us for 1.2 GB, e4m3 ones of 64: 206, 236), and so are those that several groups of query heads read (two of 32
+  // of 64/1 heads of 128: 282 instead of 327).  (One run on one box.)
   constexpr bool kWholeLines = kD * KV::kBytes % 128 == 0;
   const bool stream = kWholeLines && a.groups == 1;
 #define DA_PAGED(streaming, sixteens)                                                                              \

@@ -19,7 +19,8 @@ def kv_pages(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, *, dt
              device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
     """An empty pool: (k_pages, v_pages), each (n_pages, page_size, n_kv_heads, head_dim), views of one tensor that
     holds what a kv head has in a page in one piece, keys and values of a token side by side (the layout of the page
-    cache's slots).  dtype bf16, fp16 or fp32, or float8_e4m3fn under 16-bit queries."""
+    cache's slots).  dtype bf16, fp16 or fp32, or float8_e4m3fn under 16-bit queries.  Heads of any size can be stored;
+    :func:`paged_decode_attention` takes 64, 96, 128 and 256 channels."""
     if dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn):
         raise TypeError(f"unsupported element type {dtype}")
     if n_pages < 0 or page_size < 1 or n_kv_heads < 1 or head_dim < 1:

@@ -650,7 +650,7 @@ int da_rotate(const void *args, size_t args_bytes, void *stream);
  * p % page_size, p = positions[t]; its query, if there are any, is turned into q_out.  A token whose p is negative or
  * beyond its table row, whose sequence is none of the table's or whose page number is none of the pool's is not
  * stored (its query is turned all the same).  No two tokens of a call share a sequence and a position.
- *   k_pages, v_pages : (n_pages, page_size, n_kv_heads, head_dim), the same strides, of page_dtype: dtype, or DA_E4M3
+ *   k_pages, v_pages : (n_pages, page_size, n_kv_heads, head_dim), the same strides, no memory shared, of page_dtype: dtype, or DA_E4M3
  *                      for 16-bit rows, which are divided by their kv head's scale (NULL: 1), clamped to 448 and rounded
  *   page_table       : (n_sequences, pages_per_sequence), rows table_stride apart
  *   sequences        : (n_tokens), or NULL: token t is of sequence t
