@@ -533,39 +533,49 @@ void changed(const at::Tensor &t) {
 }
 int64_t stride_of(const at::Tensor &t, int64_t d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 bool dense_rows(const at::Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
-// Whether two tensors of the same sizes and strides have a byte in common, exactly: they lie `apart` bytes from each other,
-// and have if differences of their indices make that up to less than an element.  Axes go from the longest stride to the
-// shortest, with the differences that the shorter ones can still make up: one or two an axis, or more where strides are
-// shorter than what lies within them (then at most `budget` are looked at, and the tensors are taken to meet).
+// What indices add to an address, axis by axis from the longest stride to the shortest, in bytes.
 struct Axis {
-  int64_t stride, most;   // bytes; largest difference of its indices
+  int64_t stride, least, most;   // least and largest index, or difference of two tensors' indices
 };
-using Axes = c10::SmallVector<Axis, 4>;
-bool made_up(const Axis *axes, size_t n, int64_t apart, int64_t element, int &budget) {
-  if (n == 0) return std::abs(apart) < element;
-  int64_t within = element - 1;
-  for (size_t i = 1; i < n; ++i) within += axes[i].stride * axes[i].most;
+using Axes = c10::SmallVector<Axis, 8>;
+constexpr int kMostLookedAt = 4096;
+void longest_first(Axes &axes) {
+  std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.stride > y.stride; });
+}
+// Whether differences of indices make up for `apart` bytes, up to less than an element (`moved`: one of them is not 0).
+// One or two an axis are looked at, those that the shorter strides can still make up for, or more where strides are
+// shorter than what lies within them: `budget` at the most, behind which tensors are taken to be apart.
+bool made_up(const Axis *axes, size_t n, int64_t apart, int64_t element, bool moved, int &budget) {
+  if (n == 0) return moved && std::abs(apart) < element;
+  int64_t low = 1 - element, high = element - 1;
+  for (size_t i = 1; i < n; ++i) low -= axes[i].stride * axes[i].most, high -= axes[i].stride * axes[i].least;
   auto floored = [](int64_t x, int64_t d) { return x / d - (x % d < 0); };
-  const int64_t s = axes[0].stride, first = std::max(-axes[0].most, -floored(within + apart, s)),
-                last = std::min(axes[0].most, floored(within - apart, s));
-  for (int64_t by = first; by <= last; ++by)
-    if (--budget < 0 || made_up(axes + 1, n - 1, apart + by * s, element, budget)) return true;
+  const int64_t s = axes[0].stride, first = std::max(axes[0].least, -floored(apart - low, s)),
+                last = std::min(axes[0].most, floored(high - apart, s));
+  for (int64_t by = first; by <= last && --budget >= 0; ++by)
+    if (made_up(axes + 1, n - 1, apart + by * s, element, moved || by != 0, budget)) return true;
   return false;
 }
-Axes axes_of(const at::Tensor &t) {
+// Whether two tensors of one type and number of axes have a byte in common, at other indices if not `anywhere`.
+bool meet(const at::Tensor &a, const at::Tensor &b, bool anywhere = true) {
+  if (a.numel() == 0 || b.numel() == 0 || a.is_meta() || b.is_meta()) return false;
+  const int64_t e = a.element_size();
   Axes axes;
-  for (int64_t d = 0; d < t.dim(); ++d)
-    if (t.size(d) > 1 && t.stride(d) > 0) axes.push_back({t.stride(d) * (int64_t)t.element_size(), t.size(d) - 1});
-  std::sort(axes.begin(), axes.end(), [](const Axis &x, const Axis &y) { return x.stride > y.stride; });
-  return axes;
-}
-constexpr int kMostLookedAt = 4096;
-bool meet(const at::Tensor &a, const at::Tensor &b) {
-  if (a.numel() == 0 || a.is_meta()) return false;
-  const Axes axes = axes_of(a);
+  for (int64_t d = 0; d < a.dim(); ++d) {
+    const int64_t as = a.size(d) > 1 ? a.stride(d) * e : 0, bs = b.size(d) > 1 ? b.stride(d) * e : 0;
+    if (as == bs || as == 0 || bs == 0) {
+      if (as + bs > 0) axes.push_back({std::max(as, bs), as ? 1 - a.size(d) : 0, bs ? b.size(d) - 1 : 0});
+    } else {
+      axes.push_back({as, 1 - a.size(d), 0});
+      axes.push_back({bs, 0, b.size(d) - 1});
+    }
+  }
+  longest_first(axes);
   int budget = kMostLookedAt;
-  return made_up(axes.data(), axes.size(), (const char *)b.data_ptr() - (const char *)a.data_ptr(), a.element_size(), budget);
+  return made_up(axes.data(), axes.size(), (const char *)b.data_ptr() - (const char *)a.data_ptr(), e, anywhere, budget);
 }
+// Whether elements of a tensor share memory.
+bool folds(const at::Tensor &t) { return at::has_internal_overlap(t) == at::MemOverlap::Yes || meet(t, t, false); }
 // Whether a tensor has a byte in memory of `length` bytes that its first element is `at` bytes behind, in the same way.
 bool reached(const Axis *axes, size_t n, int64_t at, int64_t element, int64_t length, int &budget) {
   int64_t within = element - 1;   // (to the last byte, behind the axes from the second on)
@@ -575,8 +585,8 @@ bool reached(const Axis *axes, size_t n, int64_t at, int64_t element, int64_t le
   if (n == 0 || at >= 0 || end < length) return true;   // (its first or last byte is there)
   const int64_t s = axes[0].stride, first = std::max<int64_t>(0, (-within - at + s - 1) / s),
                 last = std::min(axes[0].most, (length - 1 - at) / s);
-  for (int64_t by = first; by <= last; ++by)
-    if (--budget < 0 || reached(axes + 1, n - 1, at + by * s, element, length, budget)) return true;
+  for (int64_t by = first; by <= last && --budget >= 0; ++by)
+    if (reached(axes + 1, n - 1, at + by * s, element, length, budget)) return true;
   return false;
 }
 bool reaches(const at::Tensor &t, const at::Tensor &memory) {   // (`memory` is contiguous)
@@ -585,7 +595,10 @@ bool reaches(const at::Tensor &t, const at::Tensor &memory) {   // (`memory` is 
   int64_t extent = t.element_size();
   for (int64_t d = 0; d < t.dim(); ++d) extent += (t.size(d) - 1) * t.stride(d) * (int64_t)t.element_size();
   if (at >= length || at + extent <= 0) return false;
-  const Axes axes = axes_of(t);
+  Axes axes;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) > 0) axes.push_back({t.stride(d) * (int64_t)t.element_size(), 0, t.size(d) - 1});
+  longest_first(axes);
   int budget = kMostLookedAt;
   return reached(axes.data(), axes.size(), at, t.element_size(), length, budget);
 }
@@ -784,14 +797,10 @@ PyObject *rotate(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
     not_for_gradients({&xq, xk}, "rotate_");
     for (const at::Tensor *t : {&xq, xk}) {
       if (!t) continue;
-      TORCH_CHECK_VALUE(dense_rows(*t) && at::has_internal_overlap(*t) != at::MemOverlap::Yes,
+      TORCH_CHECK_VALUE(dense_rows(*t) && !folds(*t),
                         "what is turned in place must have dense rows that do not share memory");
     }
-    if (xk) {
-      const auto overlap = at::get_overlap_status(xq, *xk);
-      TORCH_CHECK_VALUE(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial,
-                        "xq and xk share memory");
-    }
+    TORCH_CHECK_VALUE(!xk || !meet(xq, *xk), "xq and xk share memory");
     y = turn_rows(xq, xk ? *xk : at::Tensor(), positions, turn, false, true);
   } else if (at::GradMode::is_enabled() && (xq.requires_grad() || (xk && xk->requires_grad()))) {
     no_eager_graph_of(xq);

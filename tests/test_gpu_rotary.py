@@ -353,3 +353,58 @@ def test_an_output_wants_a_gradient_if_its_input_does(layout):
             v = randn(g, *d.shape, dtype=d.dtype)
             again, = torch.autograd.grad(d, (r,), v, retain_graph=True)
             check(again, v, positions, freqs, layout)
+
+
+def test_rows_in_place_that_share_memory_are_found_whatever_their_strides():
+    """Parts of a fused projection with a head in common, windows over one another; parts that only lie between each other
+    are turned."""
+    freqs, _ = rotary_frequencies(64, device=DEV)
+    positions = torch.arange(5, device=DEV)
+    fused = torch.zeros(5, 12, 64, device=DEV)
+    flat = torch.zeros(5000, device=DEV)
+    for q, k in ((fused[:, :8], fused[:, 7:10]), (fused[:, 7:], fused[:, :8]), (fused[:, ::2], fused[:, 4:5]),
+                 (fused[:, :4], fused[:, :4]), (fused[:, :4], fused[:, :4, :]), (fused, fused),
+                 (flat.as_strided((5, 4, 64), (256, 64, 1)), flat.as_strided((5, 2, 64), (300, 64, 1), 1270))):
+        with pytest.raises(ValueError, match="xq and xk share memory"):
+            rotate_(q, k, positions, freqs)
+    for q in (flat.as_strided((5, 4, 64), (64, 64, 1)), flat.as_strided((5, 4, 64), (250, 64, 1)), flat.as_strided((5, 4, 64), (256, 60, 1)),
+              fused[:, :1].expand(5, 4, 64)):
+        with pytest.raises(ValueError, match="do not share memory"):
+            rotate_(q, None, positions, freqs)
+    g = gen(13)
+    base = randn(g, 5, 12, 64, dtype=torch.float32)
+    strided = randn(g, 5000, dtype=torch.float32)
+    for q, k in ((base[:, :8], base[:, 8:]), (base[:, ::2], base[:, 1::2]), (base[:, 4:5], base[:, 5:]), (base[:, :0], base),
+                 (strided.as_strided((5, 2, 64), (320, 64, 1)), strided.as_strided((5, 3, 64), (320, 64, 1), 128)),
+                 (strided.as_strided((5, 4, 64), (64, 320, 1)), strided.as_strided((5, 2, 64), (128, 64, 1), 1600))):
+        q0, k0 = q.clone(), k.clone()
+        rotate_(q, k, positions, freqs)
+        check(q, q0, positions, freqs, "interleaved")
+        check(k, k0, positions, freqs, "interleaved")
+
+
+def test_rows_in_place_that_share_memory_are_found_exactly():
+    """Against the sets of elements, over views of any strides of one buffer."""
+    import random
+
+    rng = random.Random(5)
+    freqs, _ = rotary_frequencies(2, device=DEV)
+    buffer, numbers, met = torch.zeros(3000, device=DEV), torch.arange(3000), [0, 0]
+    for _ in range(300):
+        views = []
+        T = rng.randint(1, 4)
+        for _ in range(2):
+            shape = (T, rng.randint(1, 4), 4)
+            views.append((shape, (rng.choice([2, 4, 7, 16, 24, 100]), rng.choice([3, 4, 8, 16, 60]), 1), rng.randint(0, 120)))
+        q, k = (buffer.as_strided(*v) for v in views)
+        places = [numbers.as_strided(*v).flatten().tolist() for v in views]
+        folds, meets = any(len(set(p)) < len(p) for p in places), bool(set(places[0]) & set(places[1]))
+        met[0] += folds
+        met[1] += meets and not folds
+        at = torch.zeros(T, dtype=torch.int32, device=DEV)
+        if folds or meets:
+            with pytest.raises(ValueError, match="do not share memory" if folds else "xq and xk share memory"):
+                rotate_(q, k, at, freqs)
+        else:
+            rotate_(q, k, at, freqs)
+    assert met == [190, 33]     # (of each kind enough)
