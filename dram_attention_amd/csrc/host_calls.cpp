@@ -902,7 +902,7 @@ PyObject *paged_append(PyObject *, PyObject *const *argv, Py_ssize_t argc) {
                     " sequences of the table: say which with sequences=");
   not_for_gradients({&xk, &xv, xq, &pages.k, &pages.v, k_scale, v_scale}, "append_kv_pages_");
   for (const at::Tensor *t : {&pages.k, &pages.v})
-    TORCH_CHECK_VALUE(at::has_internal_overlap(*t) != at::MemOverlap::Yes, "pages must not share memory");
+    TORCH_CHECK_VALUE(!folds(*t), "pages must not share memory");
   TORCH_CHECK_VALUE(!meet(pages.k, pages.v), "k_pages and v_pages share memory");
   on_device_of(xk, {{&xv, "xv"}, {&pages.k, "k_pages"}, {&pages.v, "v_pages"}, {&pages.table, "page_table"},
                     {&positions, "positions"}, {sequences, "sequences"}, {xq, "xq"}, {turn.freqs, "freqs"},

@@ -357,18 +357,20 @@ def test_pools_that_share_memory_are_found_exactly():
 
     rng = random.Random(3)
     buffer = torch.zeros(4000, dtype=torch.bfloat16)
-    met = 0
+    met = [0, 0]
     for _ in range(400):
         sizes = [rng.randint(1, 4), rng.randint(1, 4), rng.randint(1, 3), rng.choice([2, 3, 8])]
         strides = [rng.choice([1, 3, 8, 12, 16, 40, 64, 200]) for _ in range(3)] + [1]
         offsets = [rng.randint(0, 200), rng.randint(0, 200)]
         pools = [buffer.as_strided(sizes, strides, at) for at in offsets]
         sets = [set(torch.arange(4000).as_strided(sizes, strides, at).flatten().tolist()) for at in offsets]
-        shared = bool(sets[0] & sets[1])
-        met += shared
-        with pytest.raises(ValueError if shared else RuntimeError, match="share memory" if shared else "GPU"):
+        folds, shared = len(sets[0]) < math.prod(sizes), bool(sets[0] & sets[1])
+        met[0] += folds
+        met[1] += shared and not folds
+        with pytest.raises(ValueError if folds or shared else RuntimeError,
+                           match="pages must not share" if folds else "k_pages and v_pages share" if shared else "GPU"):
             append_into(*pools)
-    assert 100 < met < 300
+    assert all(40 < n < 300 for n in met)
 
 
 def test_attention_refuses_to_write_over_what_it_reads():
