@@ -735,7 +735,7 @@ int launch_paged_dim(const PagedArgs &a, hipStream_t s) {
   // of e4m3 rows of 128, 94 instead of 104 for 128K tokens of bf16 ones, 146 instead of 152 for 800 MB of fp32 ones (of 256
   // 295 instead of 285 for 1.6 GB).  Rows that share lines are read faster through the caches (bf16 ones of 96: 223 instead
   // of 261 us for 1.2 GB, e4m3 ones of 64: 206, 236), and so are those that several groups of query heads read (two of 32
-  // of 64/1 heads of 128: 282 instead of 327).  (One run on one box.)
+  // of 64/1 heads of 128: 282 instead of 327).  (All from one run.)
   constexpr bool kWholeLines = kD * KV::kBytes % 128 == 0;
   const bool stream = kWholeLines && a.groups == 1;
 #define DA_PAGED(streaming, sixteens)                                                                              \
